@@ -285,6 +285,82 @@ int prism_cuda_attention_kv(prism_cuda_ctx *ctx, uint32_t layer, const uint16_t 
 int prism_cuda_attention_step_kv(prism_cuda_ctx *ctx, uint32_t layer, const uint16_t *q, const uint16_t *k,
                                  const uint16_t *v, uint64_t token_idx, uint32_t num_heads, uint32_t kv_heads,
                                  uint32_t head_dim, uint32_t rope_k, float rope_base, uint16_t *out);
+/* ---- a key/value cache of several sequences, quantised as it is written, and the attention that reads it (not in the
+ *      reference, whose KVCache is one Vec per layer, engine_impl.rs:514-530) --------------------------------------------
+ * The memory is the caller's; one prism_cache describes one layer's.  k and v are pools of pages
+ * [n_pages][kv_heads][page_size][head]: a head of a position is head_dim 16-bit values or codes; k_scale and v_scale are
+ * [n_pages][kv_heads][page_size] 32-bit numbers (4-bit codes: pairs scale, zero).  Position p of sequence s lies in page
+ * page_table[s * table_stride + p / page_size], or, without a table, in page s * table_stride + p / page_size.
+ *   PRISM_CACHE_16BIT   the rows' own type
+ *   PRISM_CACHE_INT8    value = code * scale,              scale = amax / 127,       code = rint(x * (127 / amax))
+ *   PRISM_CACHE_E4M3    value = code * scale,              scale = amax / 448,       code = nearest e4m3 to x * (448 / amax)
+ *   PRISM_CACHE_INT4    value = (code - 8) * scale + zero, scale = (hi - lo) / 15,   code = rint((x - lo) * (15 / (hi - lo))),
+ *                       zero = lo + 8 * scale; element 2i in the low half of byte i
+ * amax, lo, hi: over one head of one position; every step one rounded 32-bit operation.  A span below 2^-100 gives scale 0; a
+ * head with a value that is not finite reads back as NaN throughout.
+ * Pages, scales and rows are 16-byte aligned device memory.  The calls run on the context's stream and return; places are in
+ * device arrays, so a captured call can be replayed with others.  A place outside the cache, or whose page is not one of the
+ * pool's, is skipped, and the next synchronising call returns PRISM_E_ARG; a negative sequence or position is padding and
+ * skipped without that. */
+enum { PRISM_CACHE_16BIT = 0, PRISM_CACHE_INT8 = 1, PRISM_CACHE_E4M3 = 2, PRISM_CACHE_INT4 = 3 };
+enum { PRISM_CACHE_ROWS_F16 = 0, PRISM_CACHE_ROWS_BF16 = 1 };
+typedef struct prism_cache {
+    uint32_t format;        /* PRISM_CACHE_* */
+    uint32_t rows;          /* PRISM_CACHE_ROWS_*: type of the rows that go in and come out, and of queries and results */
+    uint32_t kv_heads, head_dim;  /* head_dim 32, 64, 128 or 256 */
+    uint32_t page_size;     /* positions of a page: a power of two, at least 16 */
+    uint32_t n_pages;       /* pages of the pool */
+    uint32_t n_seqs;        /* sequences: rows of the page table */
+    uint32_t table_stride;  /* pages of a sequence; table_stride * page_size <= 2^30 */
+    void *k, *v;
+    float *k_scale, *v_scale;   /* unused by PRISM_CACHE_16BIT */
+    const int32_t *page_table;  /* device, [n_seqs][table_stride]; NULL: n_pages >= n_seqs * table_stride */
+} prism_cache;
+
+/* Row r of k and v (kv_heads * head_dim values, k_stride / v_stride values apart, both multiples of 8) goes to position pos[r] of
+ * sequence seq[r].  The places of one call are distinct. */
+int prism_cuda_cache_write_dev(prism_cuda_ctx *ctx, const prism_cache *cache, const void *k, const void *v, uint64_t k_stride,
+                               uint64_t v_stride, uint32_t n_rows, const int32_t *seq, const int32_t *pos);
+/* The inverse: rows of the values that position pos[r] of sequence seq[r] stands for, rounded once.  Rows of skipped places are
+ * left as they were. */
+int prism_cuda_cache_read_dev(prism_cuda_ctx *ctx, const prism_cache *cache, void *k, void *v, uint64_t k_stride, uint64_t v_stride,
+                              uint32_t n_rows, const int32_t *seq, const int32_t *pos);
+/* Accepted drafted tokens: for every entry e < n_entries and j < kept[e] <= path_stride, position base[e] + path[e * path_stride + j]
+ * of sequence seq[e] moves to base[e] + j.  A path rises (path[j] >= j); entries are of distinct sequences, or of distinct pages. */
+int prism_cuda_cache_keep_dev(prism_cuda_ctx *ctx, const prism_cache *cache, uint32_t n_entries, const int32_t *seq, const int32_t *base,
+                              const int32_t *path, uint32_t path_stride, const int32_t *kept);
+
+/* Attention of the newest tokens of some sequences over their cached positions, their own included (written before).
+ * Entry e: rows q_start[e] .. q_start[e + 1] - 1 of q and out are the newest tokens of sequence seq[e], which holds length[e]
+ * positions; without a tree the last row is the one at position length[e] - 1.  A row at position p sees position c <= p if window
+ * is 0, or c > p - window, or c < sinks.
+ * With a tree the rows are drafted tokens of equal standing: row i of the entry lies at position length[e] - n + i of the cache and sees
+ * the drafted position j of its own entry if bit j of its mask (tree[row * tree_words], 64 bits a word) is set; of the committed
+ * positions c < length[e] - n it sees those that window and sinks leave to a token at q_pos[row].
+ * Query heads are shared evenly by the cached ones.  out = sum of softmax(scale * q k) v, scores, weights' sums and result in 32
+ * bits; a row that sees nothing is 0, rows of no entry (and of an entry with a negative sequence) are left as they were. */
+typedef struct prism_cache_attention {
+    const void *q;           /* rows of num_heads * head_dim values */
+    void *out;
+    uint64_t q_stride, out_stride;  /* values between rows, multiples of 8 */
+    uint32_t n_rows;         /* rows of q and out */
+    uint32_t n_entries;
+    const int32_t *seq;      /* [n_entries], device */
+    const int32_t *q_start;  /* [n_entries + 1], device */
+    const int32_t *length;   /* [n_entries], device */
+    uint32_t max_tokens;     /* no entry has more rows (an entry that has is skipped, as a bad place is) */
+    uint32_t max_length;     /* longest length to be expected: how the work is cut; a longer one is right too */
+    uint32_t num_heads;
+    uint32_t window, sinks;  /* window 0: everything is visible */
+    float scale;             /* of the scores; 0: 1 / sqrt(head_dim) */
+    const uint64_t *tree;    /* [n_rows][tree_words], device; NULL: no tree */
+    uint32_t tree_words;     /* at least (max_tokens + 63) / 64 */
+    const int32_t *q_pos;    /* [n_rows], device; read with a tree under a window */
+} prism_cache_attention;
+/* Captured calls use memory of their capture, which the context keeps; calls of one context, and replays of one capture, do not
+ * overlap. */
+int prism_cuda_cache_attention_dev(prism_cuda_ctx *ctx, const prism_cache *cache, const prism_cache_attention *a);
+
 /* argmax (engine_impl.rs:1448-1459): first strictly greatest. */
 int prism_cuda_argmax(prism_cuda_ctx *ctx, const uint16_t *logits, uint32_t n, uint32_t *index);
 

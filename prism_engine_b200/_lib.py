@@ -67,6 +67,24 @@ class CImagePlan(C.Structure):
                 ("attention_strategy", C.c_char * 24), ("lm_head_backend", C.c_char * 16)]
 
 
+class KvCache(C.Structure):
+    """Mirror of ``prism_cache``: one layer's cache in the caller's device memory (``kv_cache`` makes one)."""
+
+    _fields_ = [("format", C.c_uint32), ("rows", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("page_size", C.c_uint32), ("n_pages", C.c_uint32), ("n_seqs", C.c_uint32), ("table_stride", C.c_uint32),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("page_table", C.c_void_p)]
+
+
+class CacheAttention(C.Structure):
+    """Mirror of ``prism_cache_attention``."""
+
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_uint64), ("out_stride", C.c_uint64),
+                ("n_rows", C.c_uint32), ("n_entries", C.c_uint32), ("seq", C.c_void_p), ("q_start", C.c_void_p),
+                ("length", C.c_void_p), ("max_tokens", C.c_uint32), ("max_length", C.c_uint32), ("num_heads", C.c_uint32),
+                ("window", C.c_uint32), ("sinks", C.c_uint32), ("scale", C.c_float), ("tree", C.c_void_p),
+                ("tree_words", C.c_uint32), ("q_pos", C.c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol include/prism_cuda.h and include/prism_cuda_bench.h declare
 _vp, _i32, _u32, _u64, _sz = C.c_void_p, C.c_int32, C.c_uint32, C.c_uint64, C.c_size_t
 _cp = C.c_char_p
@@ -152,6 +170,10 @@ SIGNATURES = {
     "prism_cuda_kv_append": (C.c_int, [_vp, _u32, _vp, _vp, _u64]),
     "prism_cuda_attention_kv": (C.c_int, [_vp, _u32, _vp, _u32, _u32, _u32, _u32, _vp]),
     "prism_cuda_attention_step_kv": (C.c_int, [_vp, _u32, _vp, _vp, _vp, _u64, _u32, _u32, _u32, _u32, C.c_float, _vp]),
+    "prism_cuda_cache_write_dev": (C.c_int, [_vp, C.POINTER(KvCache), _vp, _vp, _u64, _u64, _u32, _vp, _vp]),
+    "prism_cuda_cache_read_dev": (C.c_int, [_vp, C.POINTER(KvCache), _vp, _vp, _u64, _u64, _u32, _vp, _vp]),
+    "prism_cuda_cache_keep_dev": (C.c_int, [_vp, C.POINTER(KvCache), _u32, _vp, _vp, _vp, _u32, _vp]),
+    "prism_cuda_cache_attention_dev": (C.c_int, [_vp, C.POINTER(KvCache), C.POINTER(CacheAttention)]),
     "prism_cuda_load_cimage_cached": (C.c_int, [_vp, _cp, _cp, _pu32, C.POINTER(C.c_int)]),
     "prism_cuda_cimage_plan": (C.c_int, [_vp, C.POINTER(CImagePlan)]),
 }

@@ -21,7 +21,7 @@ from typing import Dict, Optional, Tuple
 import numpy as np
 
 from . import _lib
-from ._lib import ModelConfig, PrismCudaError, check
+from ._lib import CacheAttention, KvCache, ModelConfig, PrismCudaError, check
 
 ROLE = {"q": 0, "k": 1, "v": 2, "o": 3, "gate": 4, "up": 5, "down": 6, "embed": 7, "lm_head": 8}
 
@@ -304,6 +304,36 @@ class CudaBackend:
         self._ck(self.L.prism_cuda_attention_kv(self.ctx, layer, _ptr(q), seq_len, num_heads, kv_heads, head_dim, _ptr(out)))
         return out
 
+    # -- a cache of several sequences in the caller's device memory (``kv_cache``), quantised as it is written ------
+    # Arguments are raw device addresses; the calls run on the context's stream and return.  seq, pos, q_start, length, base,
+    # path, kept and q_pos are int32 arrays on the device; strides are in values and default to rows without gaps.
+    def cache_write_dev(self, cache: KvCache, k: int, v: int, n_rows: int, seq: int, pos: int, k_stride: int = 0, v_stride: int = 0) -> None:
+        """Row r of ``k`` and ``v`` goes to position ``pos[r]`` of sequence ``seq[r]``; negative ones are padding."""
+        w = cache.kv_heads * cache.head_dim
+        self._ck(self.L.prism_cuda_cache_write_dev(self.ctx, C.byref(cache), k, v, k_stride or w, v_stride or w, n_rows, seq, pos))
+
+    def cache_read_dev(self, cache: KvCache, k: int, v: int, n_rows: int, seq: int, pos: int, k_stride: int = 0, v_stride: int = 0) -> None:
+        """Rows of the values that position ``pos[r]`` of sequence ``seq[r]`` stands for; rows of padding stay as they were."""
+        w = cache.kv_heads * cache.head_dim
+        self._ck(self.L.prism_cuda_cache_read_dev(self.ctx, C.byref(cache), k, v, k_stride or w, v_stride or w, n_rows, seq, pos))
+
+    def cache_keep_dev(self, cache: KvCache, n_entries: int, seq: int, base: int, path: int, path_stride: int, kept: int) -> None:
+        """Accepted drafted tokens: position ``base[e] + path[e, j]`` of sequence ``seq[e]`` moves to ``base[e] + j``, j < ``kept[e]``."""
+        self._ck(self.L.prism_cuda_cache_keep_dev(self.ctx, C.byref(cache), n_entries, seq, base, path, path_stride, kept))
+
+    def cache_attention_dev(self, cache: KvCache, q: int, out: int, n_rows: int, n_entries: int, seq: int, q_start: int, length: int,
+                            max_tokens: int, max_length: int, num_heads: int, window: int = 0, sinks: int = 0, scale: float = 0.0,
+                            tree: int = 0, tree_words: int = 0, q_pos: int = 0, q_stride: int = 0, out_stride: int = 0) -> None:
+        """Attention of the newest tokens of some sequences over their cached positions, their own included.  Entry e is rows
+        ``q_start[e] .. q_start[e + 1]`` of ``q`` and ``out`` over the first ``length[e]`` positions of sequence ``seq[e]``; under a
+        ``window`` a row sees that many positions up to its own and the first ``sinks``.  ``tree``: 64-bit masks (``tree_words`` a
+        row) of the drafted tokens of its entry that each row sees, itself included; ``q_pos``: the rows' positions, which a window
+        over the committed ones goes by.  ``scale`` 0: 1 / sqrt(head_dim)."""
+        w = num_heads * cache.head_dim
+        a = CacheAttention(q, out, q_stride or w, out_stride or w, n_rows, n_entries, seq, q_start, length, max_tokens, max_length, num_heads,
+                           window, sinks, scale, tree or None, tree_words, q_pos or None)
+        self._ck(self.L.prism_cuda_cache_attention_dev(self.ctx, C.byref(cache), C.byref(a)))
+
     # -- tensor parallel ------------------------------------------------------------------------------------------
     @staticmethod
     def tp_unique_id() -> bytes:
@@ -353,6 +383,23 @@ class CudaBackend:
 
     def tp_all_reduce_resid_dev(self, partial_dev: int, h_dev: int, n: int) -> None:
         self._ck(self.L.prism_cuda_tp_all_reduce_resid_dev(self.ctx, partial_dev, h_dev, n))
+
+
+CACHE_FORMATS = {"16": 0, "int8": 1, "e4m3": 2, "int4": 3}
+CACHE_ROWS = {"fp16": 0, "bf16": 1}
+
+
+def kv_cache(format: str, rows: str, kv_heads: int, head_dim: int, page_size: int, n_pages: int, n_seqs: int, table_stride: int, k: int, v: int,
+             k_scale: int = 0, v_scale: int = 0, page_table: int = 0) -> KvCache:
+    """One layer's key/value cache in the caller's device memory (``prism_cache``; addresses as ints, e.g. ``tensor.data_ptr()``).
+
+    ``k`` / ``v``: pools ``[n_pages, kv_heads, page_size, head]`` of ``rows`` values (format "16") or codes ("int8", "e4m3", "int4":
+    two in a byte); ``k_scale`` / ``v_scale``: fp32 ``[n_pages, kv_heads, page_size]``, for "int4" pairs (scale, zero).
+    ``page_table``: int32 ``[n_seqs, table_stride]`` on the device; 0: sequence s owns pages ``s * table_stride ..``."""
+    if format not in CACHE_FORMATS or rows not in CACHE_ROWS:
+        raise ValueError(f"kv_cache: format one of {sorted(CACHE_FORMATS)}, rows one of {sorted(CACHE_ROWS)}")
+    return KvCache(CACHE_FORMATS[format], CACHE_ROWS[rows], kv_heads, head_dim, page_size, n_pages, n_seqs, table_stride, k, v, k_scale or None,
+                   v_scale or None, page_table or None)
 
 
 def model_config(num_layers, hidden_size, num_heads, num_kv_heads, head_dim, intermediate_size, vocab_size,
