@@ -1,30 +1,797 @@
-// Attention of the newest tokens of some sequences over a caller-owned cache (prism_cuda_cache_attention_dev).
+// Attention of the newest tokens of some sequences over a caller-owned cache (prism_cuda_cache_attention_dev): the kernel for few
+// query rows per cached head.
+//
+// A block takes 16 query rows that share a cached head (the heads of its group, of one token or several) and a part of the
+// positions that any of them sees; its four warps take tiles of 16 or 32 positions in turn, each with its own ring of stages
+// (cp.async), running maximum and sums, so no warp waits for another before the end.  S = q K^T and O += P V are mma.sync with the
+// rows as M.  Codes go from shared memory to fragments in registers, with no 16-bit copy in between: a lane's fragments of K
+// are consecutive codes of a row (the order of a contraction is free, so q's fragments follow it), those of V are the same
+// columns of four rows, their bytes interleaved.  Codes are exact in fp16, so scales stay out of the products:
+//   score = (q c) ks + (sum of q) kz,     o = sum of (w vs) c + sum of w vz.
+// w vs enters the product as fp16 over the power of two below the largest vs so far, 2^14-fold, so no scale over- or underflows;
+// with 16-bit rows w itself does (bf16: as it is), and the sum that divides is that of the rounded weights.  q of 8- and 4-bit caches enters
+// as fp16 over a power of two.  Maxima, sums, O and everything that multiplies them are 32 bits.
+//
+// Positions past the end are zero.  A position that some row of the block does not see meets weight 0, which an infinity there turns into
+// NaN: a row whose result is not finite is taken again by itself (cache_plain_row).
+//
+// Where there are fewer rows than SMs the positions are cut into S parts; a block leaves maxima, sums and O in scratch, and the
+// last of a row tile joins them in order.
+// Bound: HBM for long caches, the latency of the chain (places, tiles, joining) for short ones.
+#include <algorithm>
 #include <cmath>
 #include <stdexcept>
+#include <vector>
 
 #include "cache_attn.cuh"
 
 namespace prism {
 
-// A warp per (row, query head), position by position.
+constexpr int CR_W = 4, CR_THREADS = CR_W * 32;  // warps of a block
+constexpr uint32_t CR_ROWS = 16, CR_MAX_SPLIT = 256;
+constexpr float CR_UP = 16384.0f;                // weights of fp16 products are 2^14-fold
 template <int KIND, int HD>
-__global__ void __launch_bounds__(128) cache_attn_plain_kernel(const CacheAttnDev a) {
+struct CrCfg {
+    static constexpr int ROWB = HD * (int)kv_bits<KIND>() / 8;
+    static constexpr int TP = ROWB >= 256 ? 16 : 32;                 // positions of a tile
+    static constexpr int NSC = (int)kv_scales<KIND>();
+    static constexpr int TILE = TP * ROWB, SCB = TP * NSC * 4;       // bytes of a tile's keys (or values), of their scales
+    static constexpr int STAGE = 2 * TILE + 2 * SCB;
+    static constexpr int ST = ROWB >= 512 ? 2 : ROWB >= 128 ? 3 : 4;
+    static constexpr int KS = HD / 16, CPL = HD / 8;                 // contraction steps of a score; columns of a lane
+    static constexpr bool Q_REGS = HD <= 128;
+    static constexpr int RING = CR_W * ST * STAGE, PARTS = CR_W * (int)CR_ROWS * HD * 4;
+    static constexpr int BODY = RING > PARTS ? RING : PARTS;         // also the warps' parts of O, and the weights of a join
+    static constexpr int Q_OFF = BODY, FRAG_OFF = Q_OFF + (int)CR_ROWS * HD * 2;  // q rows, then as fragments
+    static constexpr int ROW_OFF = FRAG_OFF + HD * 32;               // CrRow of each row, then the warps' maxima and sums
+    static constexpr size_t SMEM = ROW_OFF + 16 * 32 + CR_W * 16 * 8 + 16 * 4 + 16;
+    static_assert(BODY >= (int)(CR_MAX_SPLIT * CR_ROWS * 4), "weights of a join");
+};
+struct CrRow {
+    const uint64_t *mask;
+    int32_t last, low;
+    float mul, qsum;   // of the scores (in powers of two); the sum of q's fragments
+    uint32_t there;
+};
+static_assert(sizeof(CrRow) == 32, "rows of 32 bytes");
+
+struct CrDev {
+    CacheAttnDev a;
+    uint32_t splits, tiles;  // parts of the positions, row tiles of an entry and head
+    float *part;             // [item][split][16 HD + 32]
+    unsigned int *count;     // [item], zero between launches
+};
+
+namespace {
+
+// Byte of a 16-byte piece c of tile row r: neighbouring rows' pieces are exchanged so that the lanes that read together (K: four
+// neighbouring pieces of rows 2i and 2i + 1; V: the same columns of rows 0, 2, 4, 6 apart) lie in different banks.
+template <int ROWB>
+__device__ __forceinline__ uint32_t cr_at(uint32_t r, uint32_t c) {
+    if constexpr (ROWB == 512) return r * 512 + ((c ^ (((r >> 1) & 3) ^ ((r & 1) << 2))) << 4);
+    else if constexpr (ROWB == 256) return r * 256 + ((c ^ ((((r >> 1) & 1) | ((r >> 2) & 1) << 2) ^ ((r & 1) << 2))) << 4);
+    else if constexpr (ROWB == 128) return r * 128 + ((c ^ (((r >> 1) & 3) << 1 ^ ((r & 1) << 2))) << 4);
+    else if constexpr (ROWB == 64) return (r >> 1) * 128 + ((r ^ (r >> 1)) & 1) * 64 + ((c ^ (((r >> 2) & 1) << 1)) << 4);
+    else if constexpr (ROWB == 32) return ((r >> 3) * 2 + (r & 1)) * 128 + ((((r >> 1) & 3) ^ ((r & 1) << 1)) << 5) + (c << 4);
+    else return r * 16;
+}
+// Place of slot j (of 4) of step ks in a head, for lane t of four: what the fragments of a row's codes hold.
+template <int KIND, int HD>
+__device__ __forceinline__ uint32_t cr_elem(uint32_t ks, uint32_t t, uint32_t j) {
+    constexpr uint32_t LB = HD * kv_bits<KIND>() / 32;  // a lane's bytes of a row
+    const uint32_t word = KIND <= KV_BF16 ? 2 * ks : KIND == KV_INT4 ? ks >> 1 : ks;
+    const uint32_t byte = LB >= 16 ? (t + 4 * (word >> 2)) * 16 + (word & 3) * 4 : t * LB + word * 4;
+    if (KIND <= KV_BF16) return byte / 2 + j;
+    if (KIND == KV_INT4) return byte * 2 + ((ks & 1) << 1) + (j >> 1) + ((j & 1) << 2);
+    return byte + j;
+}
+
+__device__ __forceinline__ float cr_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool BF16>
+__device__ __forceinline__ void cr_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Bytes copied, the rest of the 16 zero.
+__device__ __forceinline__ void cr_cp16(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cr_lds(uint32_t (&w)[N], uint32_t at) {
+    if constexpr (N == 4) asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+    else if constexpr (N == 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+    else asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w[0]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t cr_lds16(uint32_t at) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t cr_sub2(uint32_t h, uint32_t what) {
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&h), *reinterpret_cast<const __half2 *>(&what));
+    return *reinterpret_cast<const uint32_t *>(&d);
+}
+// Four 8-bit codes as two fp16 pairs.
+template <int KIND>
+__device__ __forceinline__ void cr_bytes(uint32_t w, uint32_t &h0, uint32_t &h1) {
+    if constexpr (KIND == KV_INT8) {
+        const uint32_t x = w ^ 0x80808080u;  // code + 128 in the low bits of 1024
+        h0 = cr_sub2(__byte_perm(x, 0x64646464u, 0x4140), 0x64806480u);
+        h1 = cr_sub2(__byte_perm(x, 0x64646464u, 0x4342), 0x64806480u);
+    } else {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}\n" : "=r"(h0), "=r"(h1) : "r"(w));
+    }
+}
+// Codes 0..7 of a word as fp16 pairs (0, 4), (1, 5), (2, 6), (3, 7), less 8.
+__device__ __forceinline__ void cr_nibbles(uint32_t w, uint32_t (&h)[4]) {
+    const uint32_t sixteenth = 0x2C002C00u, off = 0xD480D480u;  // 1 / 16, -(64 + 8)
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t x = w >> (8 * i);
+        h[2 * i] = cr_sub2((x & 0x000F000Fu) | 0x64006400u, 0x64086408u);
+        const uint32_t y = (x & 0x00F000F0u) | 0x64006400u;
+        const __half2 d = __hfma2(*reinterpret_cast<const __half2 *>(&y), *reinterpret_cast<const __half2 *>(&sixteenth), *reinterpret_cast<const __half2 *>(&off));
+        h[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&d);
+    }
+}
+__device__ __forceinline__ float cr_pow2_below(float x) { return __uint_as_float(min(__float_as_uint(x) & 0x7F800000u, 253u << 23)); }
+__device__ __forceinline__ float cr_inv_pow2(float p) { return p > 0.0f ? __uint_as_float((254u << 23) - __float_as_uint(p)) : 0.0f; }
+
+}  // namespace
+
+template <int KIND, int HD>
+__global__ void __launch_bounds__(CR_THREADS) cache_rows_kernel(const __grid_constant__ CrDev d) {
+    using C = CrCfg<KIND, HD>;
+    constexpr int TP = C::TP, NT = TP / 8, KS = C::KS, CPL = C::CPL, ROWB = C::ROWB, NSC = C::NSC, ST = C::ST;
+    constexpr bool CODES = KIND >= KV_INT8, BF16 = KIND == KV_BF16;
+    const CacheAttnDev &a = d.a;
+    extern __shared__ __align__(128) uint8_t cr_smem[];
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t unit = blockIdx.x * 4 + (threadIdx.x >> 5), token = unit / a.heads, head = unit % a.heads;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const uint32_t item = blockIdx.x / d.splits, split = blockIdx.x - item * d.splits;
+    const uint32_t tile = item % d.tiles, kh = item / d.tiles % a.c.kv_heads, e = item / d.tiles / a.c.kv_heads;
     CacheEntry x;
-    if (!cache_entry(a, blockIdx.y, x) || token >= x.n) return;
-    cache_plain_row<KIND, HD>(a, x, token, head, threadIdx.x & 31);
+    if (!cache_entry(a, e, x)) return;                     // the same in all blocks of an item
+    const uint32_t n_rows = x.n * a.group, r0 = tile * CR_ROWS;
+    if (r0 >= n_rows) return;
+    const uint32_t here = min(CR_ROWS, n_rows - r0), tok_lo = r0 / a.group, tok_hi = (r0 + here - 1) / a.group;
+
+    CrRow *rows = reinterpret_cast<CrRow *>(cr_smem + C::ROW_OFF);
+    float *w_max = reinterpret_cast<float *>(cr_smem + C::ROW_OFF + 16 * 32), *w_sum = w_max + CR_W * 16, *r_sum = w_sum + CR_W * 16;
+    uint32_t *flags = reinterpret_cast<uint32_t *>(r_sum + 16);  // rows to be taken again; whether this block joins
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(cr_smem) + warp * ST * C::STAGE;
+
+    // ---- the positions that some row sees: the first tiles (a.sinks), then main_lo .. ---------------------------------
+    int32_t low = x.len, low_max = -1;
+    if (!a.window) low = -1;
+    else if (!a.tree) {
+        low = cache_row(a, x, tok_lo).low;
+        low_max = cache_row(a, x, tok_hi).low;
+    } else {
+        for (uint32_t i = tok_lo; i <= tok_hi; i++) {
+            const int32_t l = cache_row(a, x, i).low;
+            low = min(low, l);
+            low_max = max(low_max, l);
+        }
+    }
+    const int32_t end = a.tree ? x.len : min(x.len, x.first + (int32_t)tok_hi + 1);  // may be negative: nothing is seen
+    const int32_t all_to = a.tree ? x.first - 1 : x.first + (int32_t)tok_lo;         // every row's last
+    const int32_t start = a.tree ? min(low + 1, max(x.first, 0)) : low + 1;
+    const uint32_t first_tiles = end > 0 ? (min((uint32_t)end, a.sinks) + TP - 1) / TP : 0;
+    const uint32_t main_lo = max((uint32_t)start / TP, first_tiles), main_hi = end > 0 ? ((uint32_t)end + TP - 1) / TP : 0;
+    const uint32_t n_tiles = first_tiles + (main_hi > main_lo ? main_hi - main_lo : 0);
+    const uint32_t i_lo = (uint32_t)((uint64_t)n_tiles * split / d.splits), i_hi = (uint32_t)((uint64_t)n_tiles * (split + 1) / d.splits);
+    auto pos_of = [&](uint32_t i) { return (int32_t)((i < first_tiles ? i : main_lo + (i - first_tiles)) * TP); };
+
+    auto fetch = [&](uint32_t i, uint32_t st) {
+        if (i < i_hi) {
+            const uint32_t kt = ring + st * C::STAGE, vt = kt + C::TILE, ksc = vt + C::TILE, vsc = ksc + C::SCB;
+            const int32_t p0 = pos_of(i);
+#pragma unroll
+            for (int u = 0; u < TP / 16; u++) {            // a page holds at least 16 positions
+                const int32_t p = p0 + u * 16;
+                uint32_t page = 0;
+                const int32_t left = p < x.len && kv_page(a.c, x.seq, (uint32_t)p, page) ? x.len - p : 0;
+                const size_t row = left ? kv_row(a.c, page, kh, (uint32_t)p) : 0;
+                const uint8_t *ks = a.c.k + row * ROWB, *vs = a.c.v + row * ROWB;
+#pragma unroll
+                for (int m = 0; m < (ROWB + 31) / 32; m++) {
+                    const uint32_t piece = m * 32 + lane, r = piece / (ROWB / 16), c = piece % (ROWB / 16), at = cr_at<ROWB>(u * 16 + r, c);
+                    if (ROWB >= 32 || piece < (uint32_t)ROWB) {
+                        const uint32_t bytes = (int32_t)r < left ? 16 : 0;
+                        cr_cp16(kt + at, ks + piece * 16, bytes);
+                        cr_cp16(vt + at, vs + piece * 16, bytes);
+                    }
+                }
+                if constexpr (NSC > 0) {
+                    constexpr uint32_t PER = 4 * NSC;      // pieces of 16 positions' scales
+                    if (lane < 2 * PER) {
+                        const uint32_t which = lane / PER, piece = lane % PER, mine = piece * (4 / NSC);  // first position of the piece
+                        const uint32_t bytes = (uint32_t)max(0, min(16, (left - (int32_t)mine) * 4 * NSC));
+                        cr_cp16((which ? vsc : ksc) + u * 64 * NSC + piece * 16, (which ? a.c.vs : a.c.ks) + row * NSC + piece * 4, bytes);
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; s++) fetch(i_lo + warp + s * CR_W, s);
+
+    // ---- rows and q's fragments -----------------------------------------------------------------------------------------
+    {
+        constexpr int PER = HD / 8;                        // values of a thread: eight threads a row
+        const uint32_t r = tid >> 3, part = tid & 7, token = (r0 + r) / a.group;
+        const bool there = r < here;
+        uint32_t w[PER / 2];
+#pragma unroll
+        for (int i = 0; i < PER / 2; i++) w[i] = 0;
+        if (there) {
+            const uint16_t *src = a.q + (size_t)(x.row0 + token) * a.q_stride + (size_t)(kh * a.group + (r0 + r) % a.group) * HD + part * PER;
+            if constexpr (PER >= 8) {
+#pragma unroll
+                for (int i = 0; i < PER / 8; i++) reinterpret_cast<uint4 *>(w)[i] = reinterpret_cast<const uint4 *>(src)[i];
+            } else {
+                *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(src);
+            }
+        }
+        float mul = a.scale * 1.4426950408889634f, sum = 0.0f;
+        if constexpr (CODES) {
+            float v[PER], big = 0.0f;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                v[i] = kv_row_value((uint16_t)(w[i >> 1] >> (16 * (i & 1))), a.c.rows_bf16);
+                big = fmaxf(big, fabsf(v[i]));
+            }
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+            const float unit = cr_pow2_below(big), inv = unit > 0.0f ? cr_inv_pow2(unit) : 1.0f;
+            if (unit > 0.0f) mul *= unit;
+#pragma unroll
+            for (int i = 0; i < PER / 2; i++) {
+                const __half2 h = __floats2half2_rn(v[2 * i] * inv, v[2 * i + 1] * inv);
+                const float2 f = __half22float2(h);
+                sum += f.x + f.y;
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        }
+        uint32_t *dst = reinterpret_cast<uint32_t *>(cr_smem + C::Q_OFF) + (r * HD + part * PER) / 2;
+#pragma unroll
+        for (int i = 0; i < PER / 2; i++) dst[i] = w[i];
+        if (part == 0) {
+            CrRow y{nullptr, -1, -1, mul, sum, there};
+            if (there) {
+                const CacheRow c = cache_row(a, x, token);
+                y.mask = c.mask;
+                y.last = c.last;
+                y.low = c.low;
+            }
+            rows[r] = y;
+        }
+        if (tid == 0) flags[0] = 0;
+    }
+    __syncthreads();
+    {
+        const uint16_t *q = reinterpret_cast<const uint16_t *>(cr_smem + C::Q_OFF);
+        uint4 *frag = reinterpret_cast<uint4 *>(cr_smem + C::FRAG_OFF);
+        for (uint32_t s = tid; s < KS * 32; s += CR_THREADS) {
+            const uint32_t ks = s >> 5, ln = s & 31, fg = ln >> 2, ft = ln & 3;
+            uint32_t el[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) el[j] = cr_elem<KIND, HD>(ks, ft, j);
+            auto pair = [&](uint32_t r, int j) { return (uint32_t)q[r * HD + el[j]] | (uint32_t)q[r * HD + el[j + 1]] << 16; };
+            frag[s] = make_uint4(pair(fg, 0), pair(fg + 8, 0), pair(fg, 2), pair(fg + 8, 2));
+        }
+    }
+    __syncthreads();
+    const uint32_t frag_at = (uint32_t)__cvta_generic_to_shared(cr_smem) + C::FRAG_OFF + lane * 16;
+    uint32_t qf[C::Q_REGS ? KS : 1][4];
+    if constexpr (C::Q_REGS) {
+#pragma unroll
+        for (int k = 0; k < KS; k++) cr_lds<4>(qf[k], frag_at + k * 512);
+    }
+    const CrRow ra = rows[g], rb = rows[g + 8];
+
+    // ---- this warp's tiles ------------------------------------------------------------------------------------------------
+    float o[CPL][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, z[2] = {0.0f, 0.0f}, unit = 0.0f;
+#pragma unroll
+    for (int i = 0; i < CPL; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) o[i][c] = 0.0f;
+    uint32_t st = 0;
+    for (uint32_t i = i_lo + warp; i < i_hi; i += CR_W) {
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(ST - 2) : "memory");
+        __syncwarp();                                      // and the whole warp is done with the tile before
+        fetch(i + (ST - 1) * CR_W, st == 0 ? ST - 1 : st - 1);
+        const uint32_t kt = ring + st * C::STAGE, vt = kt + C::TILE, ksc = vt + C::TILE, vsc = ksc + C::SCB;
+        const int32_t p0 = pos_of(i);
+        // scores
+        float s[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) s[j][c] = 0.0f;
+            const uint32_t r = j * 8 + g;
+            auto step = [&](int k, uint32_t b0, uint32_t b1) {
+                if constexpr (C::Q_REGS) {
+                    cr_mma<BF16>(s[j], qf[k], b0, b1);
+                } else {
+                    uint32_t q4[4];
+                    cr_lds<4>(q4, frag_at + k * 512);
+                    cr_mma<BF16>(s[j], q4, b0, b1);
+                }
+            };
+            constexpr int LB = ROWB / 4, NW = LB >= 16 ? 4 : LB / 4;  // a lane's bytes of a row, words of an access
+#pragma unroll
+            for (int pc = 0; pc < (LB + 15) / 16; pc++) {
+                uint32_t w[NW];
+                if constexpr (LB >= 16) cr_lds<NW>(w, kt + cr_at<ROWB>(r, t + 4 * pc));
+                else if constexpr (LB == 8) cr_lds<NW>(w, kt + cr_at<ROWB>(r, t >> 1) + (t & 1) * 8);
+                else cr_lds<NW>(w, kt + cr_at<ROWB>(r, 0) + t * 4);
+                if constexpr (KIND <= KV_BF16) {
+#pragma unroll
+                    for (int q = 0; q < NW / 2; q++) step(pc * 2 + q, w[2 * q], w[2 * q + 1]);
+                } else if constexpr (KIND == KV_INT4) {
+#pragma unroll
+                    for (int q = 0; q < NW; q++) {
+                        uint32_t h[4];
+                        cr_nibbles(w[q], h);
+                        step((pc * 4 + q) * 2, h[0], h[1]);
+                        step((pc * 4 + q) * 2 + 1, h[2], h[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < NW; q++) {
+                        uint32_t h0, h1;
+                        cr_bytes<KIND>(w[q], h0, h1);
+                        step(pc * 4 + q, h0, h1);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            if constexpr (NSC == 2) {
+                uint32_t w[4];
+                cr_lds<4>(w, ksc + (j * 8 + 2 * t) * 8);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const float sc = __uint_as_float(w[(c & 1) * 2]), zero = __uint_as_float(w[(c & 1) * 2 + 1]);
+                    s[j][c] = fmaf(s[j][c], sc, (c < 2 ? ra.qsum : rb.qsum) * zero);
+                }
+            } else if constexpr (NSC == 1) {
+                uint32_t w[2];
+                cr_lds<2>(w, ksc + (j * 8 + 2 * t) * 4);
+#pragma unroll
+                for (int c = 0; c < 4; c++) s[j][c] *= __uint_as_float(w[c & 1]);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; c++) s[j][c] *= c < 2 ? ra.mul : rb.mul;
+        }
+        const bool whole = p0 + TP - 1 <= all_to && (p0 > low_max || (uint32_t)(p0 + TP) <= a.sinks);
+        if (!whole) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const CrRow &r = c < 2 ? ra : rb;
+                uint32_t seen = 0;                         // a bit for each of the lane's columns
+                uint64_t bits = 0;
+                int32_t from = 0;                          // drafted position of bit 0
+                if (a.tree && r.mask && p0 + TP > x.first) {
+                    from = max(p0 - x.first, 0);
+                    bits = __ldg(r.mask + (from >> 6)) >> (from & 63);
+                    if ((from & 63) && (from >> 6) + 1 < (int32_t)a.tree_words) bits |= __ldg(r.mask + (from >> 6) + 1) << (64 - (from & 63));
+                }
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    const int32_t p = p0 + j * 8 + 2 * t + (c & 1);
+                    bool see = p <= r.last && (p > r.low || (uint32_t)p < a.sinks);
+                    if (a.tree && p >= x.first) see = r.mask && p < x.len && (bits >> (p - x.first - from) & 1);
+                    seen |= (uint32_t)see << j;
+                }
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+                    if (!(seen >> j & 1)) s[j][c] = -INFINITY;
+            }
+        }
+        // weights
+        float alpha[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float top = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
+#pragma unroll
+            for (int j = 1; j < NT; j++) top = fmaxf(top, fmaxf(s[j][2 * h], s[j][2 * h + 1]));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            top = fmaxf(top, m[h]);
+            float sub = top == -INFINITY ? 0.0f : top;     // nothing but scores of -inf so far: weights 0
+            alpha[h] = cr_ex2(m[h] - sub);
+            m[h] = top;
+            l[h] *= alpha[h];
+            z[h] *= alpha[h];
+            if (KIND == KV_F16) sub -= 14.0f;
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) s[j][2 * h + c] = cr_ex2(s[j][2 * h + c] - sub);
+        }
+        uint32_t pf[NT][2];                                // rows g and g + 8, columns 2t and 2t + 1 of each 8
+        if constexpr (CODES) {
+            float vs[NT][2], vz[NT][2], top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                if constexpr (NSC == 2) {
+                    uint32_t w[4];
+                    cr_lds<4>(w, vsc + (j * 8 + 2 * t) * 8);
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        vs[j][c] = __uint_as_float(w[2 * c]);
+                        vz[j][c] = __uint_as_float(w[2 * c + 1]);
+                    }
+                } else {
+                    uint32_t w[2];
+                    cr_lds<2>(w, vsc + (j * 8 + 2 * t) * 4);
+#pragma unroll
+                    for (int c = 0; c < 2; c++) vs[j][c] = __uint_as_float(w[c]);
+                }
+                top = fmaxf(top, fmaxf(fabsf(vs[j][0]), fabsf(vs[j][1])));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            const float next = fmaxf(unit, cr_pow2_below(top)), inv = cr_inv_pow2(next), f = unit * inv;  // next > 0 unless all scales were 0
+            if (next != unit) {
+                alpha[0] *= f;
+                alpha[1] *= f;
+                unit = next;
+            }
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    l[h] += s[j][2 * h] + s[j][2 * h + 1];
+                    if constexpr (NSC == 2) z[h] = fmaf(s[j][2 * h], vz[j][0], fmaf(s[j][2 * h + 1], vz[j][1], z[h]));
+                    const __half2 p = __floats2half2_rn(s[j][2 * h] * (vs[j][0] * inv * CR_UP), s[j][2 * h + 1] * (vs[j][1] * inv * CR_UP));
+                    pf[j][h] = *reinterpret_cast<const uint32_t *>(&p);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if constexpr (BF16) {
+                        const __nv_bfloat162 p = __floats2bfloat162_rn(s[j][2 * h], s[j][2 * h + 1]);
+                        pf[j][h] = *reinterpret_cast<const uint32_t *>(&p);
+                        l[h] += __uint_as_float(pf[j][h] << 16) + __uint_as_float(pf[j][h] & 0xFFFF0000u);
+                    } else {
+                        const __half2 p = __floats2half2_rn(s[j][2 * h], s[j][2 * h + 1]);
+                        pf[j][h] = *reinterpret_cast<const uint32_t *>(&p);
+                        const float2 b = __half22float2(p);
+                        l[h] += b.x + b.y;
+                    }
+                }
+        }
+        if (__any_sync(0xFFFFFFFFu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+            for (int c = 0; c < CPL; c++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) o[c][q] *= alpha[q >> 1];
+        }
+        // O += P V, 16 positions at a time
+#pragma unroll
+        for (int kk = 0; kk < TP / 16; kk++) {
+            const uint32_t pa[4] = {pf[2 * kk][0], pf[2 * kk][1], pf[2 * kk + 1][0], pf[2 * kk + 1][1]};
+            const uint32_t r[4] = {kk * 16 + 2 * t, kk * 16 + 2 * t + 1, kk * 16 + 2 * t + 8, kk * 16 + 2 * t + 9};
+            constexpr int CB = ROWB / 8, NW = CB >= 16 ? 4 : CB >= 4 ? CB / 4 : 1;  // a lane's bytes of a row, words of an access
+#pragma unroll
+            for (int pc = 0; pc < (CB + 15) / 16; pc++) {
+                uint32_t w[4][NW];
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    if constexpr (CB >= 16) cr_lds<NW>(w[q], vt + cr_at<ROWB>(r[q], g * (CB / 16) + pc));
+                    else if constexpr (CB == 8) cr_lds<NW>(w[q], vt + cr_at<ROWB>(r[q], g >> 1) + (g & 1) * 8);
+                    else if constexpr (CB == 4) cr_lds<NW>(w[q], vt + cr_at<ROWB>(r[q], g >> 2) + (g & 3) * 4);
+                    else w[q][0] = cr_lds16(vt + cr_at<ROWB>(r[q], 0) + g * 2);
+                }
+#pragma unroll
+                for (int v = 0; v < NW; v++) {
+                    if constexpr (KIND <= KV_BF16) {
+                        const int c = (pc * 4 + v) * 2;
+                        cr_mma<BF16>(o[c], pa, __byte_perm(w[0][v], w[1][v], 0x5410), __byte_perm(w[2][v], w[3][v], 0x5410));
+                        cr_mma<BF16>(o[c + 1], pa, __byte_perm(w[0][v], w[1][v], 0x7632), __byte_perm(w[2][v], w[3][v], 0x7632));
+                    } else if constexpr (KIND == KV_INT4) {
+#pragma unroll
+                        for (int half = 0; half < (CB == 2 ? 1 : 2); half++) {
+                            const int c = (pc * 4 + v) * 8 + half * 4;
+                            uint32_t b0[4], b1[4];
+                            cr_nibbles(__byte_perm(w[0][v], w[1][v], half ? 0x7632 : 0x5410), b0);
+                            cr_nibbles(__byte_perm(w[2][v], w[3][v], half ? 0x7632 : 0x5410), b1);
+#pragma unroll
+                            for (int q = 0; q < 4; q++) cr_mma<false>(o[c + q], pa, b0[q], b1[q]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int half = 0; half < 2; half++) {
+                            const int c = (pc * 4 + v) * 4 + half * 2;
+                            uint32_t b0[2], b1[2];
+                            cr_bytes<KIND>(__byte_perm(w[0][v], w[1][v], half ? 0x7362 : 0x5140), b0[0], b0[1]);
+                            cr_bytes<KIND>(__byte_perm(w[2][v], w[3][v], half ? 0x7362 : 0x5140), b1[0], b1[1]);
+#pragma unroll
+                            for (int q = 0; q < 2; q++) cr_mma<false>(o[c + q], pa, b0[q], b1[q]);
+                        }
+                    }
+                }
+            }
+        }
+        st = st + 1 == ST ? 0 : st + 1;
+    }
+    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+
+    // ---- the warps' parts, in the order of fragments: value [column][4][lane] -----------------------------------------------
+    __syncthreads();                                       // the rings are free
+    float *parts = reinterpret_cast<float *>(cr_smem), *sum_of = parts;  // the first warp's place takes the sum
+    constexpr uint32_t VALUES = CR_ROWS * HD;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
+        if constexpr (NSC == 2) {
+            z[h] += __shfl_xor_sync(0xFFFFFFFFu, z[h], 1);
+            z[h] += __shfl_xor_sync(0xFFFFFFFFu, z[h], 2);
+        }
+        if (t == 0) {
+            w_max[warp * 16 + g + 8 * h] = m[h];
+            w_sum[warp * 16 + g + 8 * h] = l[h];
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < CPL; c++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            float v = o[c][q];
+            if constexpr (CODES) v = v * (1.0f / CR_UP) * unit;
+            if constexpr (NSC == 2) v += z[q >> 1];
+            parts[warp * VALUES + (c * 4 + q) * 32 + lane] = v;
+        }
+    __syncthreads();
+    {
+        const uint32_t used = min((uint32_t)CR_W, i_hi - i_lo);  // warps that had a tile
+        float top[2], f[CR_W][2], sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            top[h] = -INFINITY;
+            for (int w = 0; w < CR_W; w++) top[h] = fmaxf(top[h], w_max[w * 16 + g + 8 * h]);
+            const float sub = top[h] == -INFINITY ? 0.0f : top[h];
+#pragma unroll
+            for (int w = 0; w < CR_W; w++) {
+                f[w][h] = cr_ex2(w_max[w * 16 + g + 8 * h] - sub);
+                sum[h] += w_sum[w * 16 + g + 8 * h] * f[w][h];
+            }
+        }
+        __syncthreads();
+        if (warp == 0 && t == 0) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                w_max[g + 8 * h] = top[h];
+                r_sum[g + 8 * h] = sum[h];
+            }
+        }
+        for (uint32_t b = warp; b < (uint32_t)CPL * 4; b += CR_W) {
+            const uint32_t h = b >> 1 & 1;
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < CR_W; w++)
+                if ((uint32_t)w < used) v += parts[w * VALUES + b * 32 + lane] * (h ? f[w][1] : f[w][0]);
+            sum_of[b * 32 + lane] = v;                     // read by this thread only, before
+        }
+    }
+    __syncthreads();
+
+    // ---- the blocks' parts ---------------------------------------------------------------------------------------------------
+    if (d.splits > 1) {
+        float *mine = d.part + (size_t)blockIdx.x * (VALUES + 32);
+        const uint32_t live = here > 8 ? 4 : 2;            // fragments of rows 8.. only where there are any
+        for (uint32_t i = tid; i < VALUES / 4; i += CR_THREADS)
+            if ((i >> 3 & 3) < live) __stcg(reinterpret_cast<float4 *>(mine) + i, reinterpret_cast<const float4 *>(sum_of)[i]);
+        if (tid < 16) {
+            __stcg(mine + VALUES + tid, w_max[tid]);
+            __stcg(mine + VALUES + 16 + tid, r_sum[tid]);
+        }
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+            const bool last = atomicAdd(d.count + item, 1u) == d.splits - 1;
+            if (last) d.count[item] = 0;                   // for the next launch
+            flags[1] = last;
+        }
+        __syncthreads();
+        if (!flags[1]) return;
+        __threadfence();
+        const float *all = d.part + (size_t)item * d.splits * (VALUES + 32);
+        float *wgt = parts;                                // [split][16]
+        {
+            const uint32_t r = tid >> 3, k = tid & 7;
+            float top = -INFINITY, sum = 0.0f;
+            for (uint32_t s = k; s < d.splits; s += 8) top = fmaxf(top, __ldcg(all + (size_t)s * (VALUES + 32) + VALUES + r));
+#pragma unroll
+            for (int q = 4; q > 0; q >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, q));
+            const float sub = top == -INFINITY ? 0.0f : top;
+            for (uint32_t s = k; s < d.splits; s += 8) {
+                const float *p = all + (size_t)s * (VALUES + 32) + VALUES + r;
+                const float f = cr_ex2(__ldcg(p) - sub);
+                wgt[s * 16 + r] = f;
+                sum += __ldcg(p + 16) * f;
+            }
+#pragma unroll
+            for (int q = 4; q > 0; q >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, q);
+            if (k == 0) r_sum[r] = sum;
+        }
+        __syncthreads();
+        constexpr int PER = VALUES / 4 / CR_THREADS > 0 ? VALUES / 4 / CR_THREADS : 1;
+        float4 acc[PER];
+#pragma unroll
+        for (int q = 0; q < PER; q++) acc[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (uint32_t s = 0; s < d.splits; s++) {
+            const float4 *p = reinterpret_cast<const float4 *>(all + (size_t)s * (VALUES + 32));
+#pragma unroll
+            for (int q = 0; q < PER; q++) {
+                const uint32_t i = q * CR_THREADS + tid, row = (i & 7) + (i >> 4 & 1) * 8;  // four lanes of one row
+                if ((i >> 3 & 3) < live) {
+                    const float4 v = __ldcg(p + i);
+                    const float f = wgt[s * 16 + row];
+                    acc[q].x = fmaf(v.x, f, acc[q].x);
+                    acc[q].y = fmaf(v.y, f, acc[q].y);
+                    acc[q].z = fmaf(v.z, f, acc[q].z);
+                    acc[q].w = fmaf(v.w, f, acc[q].w);
+                }
+            }
+        }
+        __syncthreads();                                   // the weights have been read
+#pragma unroll
+        for (int q = 0; q < PER; q++) reinterpret_cast<float4 *>(sum_of)[q * CR_THREADS + tid] = acc[q];
+        __syncthreads();
+    }
+
+    // ---- results: eight columns of a row a thread ----------------------------------------------------------------------------
+    constexpr uint32_t COLS = CPL >= 8 ? 8 : 4;            // consecutive columns that a thread stores
+    for (uint32_t u = tid; u < VALUES / COLS; u += CR_THREADS) {
+        const uint32_t ln = u & 31, q = u >> 5 & 3, c0 = (u >> 7) * COLS, r = (ln >> 2) + (q >> 1) * 8;
+        if (r >= here) continue;
+        const float sum = r_sum[r], inv = 1.0f / sum;
+        float v[COLS];
+        bool odd = !(sum > 0.0f);
+#pragma unroll
+        for (uint32_t i = 0; i < COLS; i++) {
+            v[i] = sum_of[((c0 + i) * 4 + q) * 32 + ln] * inv;
+            odd |= !isfinite(v[i]);
+        }
+        if (odd) {
+            atomicOr(flags, 1u << r);
+            continue;
+        }
+        const uint32_t rr = r0 + r, col = (2 * (ln & 3) + (q & 1)) * CPL + c0;
+        uint16_t *dst = a.out + (size_t)(x.row0 + rr / a.group) * a.out_stride + (size_t)(kh * a.group + rr % a.group) * HD + col;
+        uint32_t w[COLS / 2];
+#pragma unroll
+        for (uint32_t i = 0; i < COLS / 2; i++) w[i] = kv_round2(v[2 * i], v[2 * i + 1], a.c.rows_bf16);
+        if constexpr (COLS == 8) *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        else *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+    }
+    __syncthreads();
+    const uint32_t again = flags[0];
+    for (uint32_t r = warp; r < here; r += CR_W)
+        if (again >> r & 1) cache_plain_row<KIND, HD>(a, x, (r0 + r) / a.group, kh * a.group + (r0 + r) % a.group, lane);
+}
+
+// ---- scratch -----------------------------------------------------------------------------------------------------------------
+// Parts and counters.  Eager calls of a context share a block, which grows when the stream is idle.  Calls that are being captured use
+// a block of their capture, kept until the context goes: a replay finds it whatever ran in between, and no two captures share one.
+struct CacheScratch {
+    struct Block {
+        unsigned long long capture;  // 0: eager
+        uint8_t *mem;
+        size_t part_bytes, counts;
+    };
+    std::vector<Block> blocks;
+};
+void cache_scratch_free(CacheScratch *s) {
+    if (!s) return;
+    for (auto &b : s->blocks) cudaFree(b.mem);
+    delete s;
+}
+static int cache_scratch(prism_cuda_ctx *ctx, size_t part_bytes, size_t counts, float **part, unsigned int **count) {
+    if (!ctx->cache_scratch) ctx->cache_scratch = new CacheScratch();
+    auto &blocks = ctx->cache_scratch->blocks;
+    cudaStreamCaptureStatus status;
+    unsigned long long id = 0;
+    PRISM_CUDA_TRY(ctx, cudaStreamGetCaptureInfo(ctx->stream, &status, &id));
+    if (status == cudaStreamCaptureStatusNone) id = 0;
+    for (size_t i = 0; i < blocks.size(); i++) {
+        auto &b = blocks[i];
+        if (b.capture != id) continue;
+        if (b.part_bytes >= part_bytes && b.counts >= counts) {
+            *part = reinterpret_cast<float *>(b.mem);
+            *count = reinterpret_cast<unsigned int *>(b.mem + b.part_bytes);
+            return PRISM_OK;
+        }
+        if (id == 0) {
+            PRISM_CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream));
+            part_bytes = std::max(part_bytes, b.part_bytes);
+            counts = std::max(counts, b.counts);
+            cudaFree(b.mem);
+            blocks.erase(blocks.begin() + i);
+            break;
+        }
+    }
+    blocks.reserve(blocks.size() + 1);                     // nothing throws between the allocation and its place
+    part_bytes = (part_bytes + 255) / 256 * 256;
+    counts = (counts + 63) / 64 * 64;
+    CacheScratch::Block b{id, nullptr, part_bytes, counts};
+    if (id == 0) {
+        PRISM_CUDA_TRY(ctx, device_malloc(ctx, (void **)&b.mem, part_bytes + counts * 4));
+    } else {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // an allocation is no part of the capture
+        PRISM_CUDA_TRY(ctx, cudaThreadExchangeStreamCaptureMode(&mode));
+        const cudaError_t e = cudaMalloc((void **)&b.mem, part_bytes + counts * 4);
+        (void)cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) {
+            (void)cudaGetLastError();
+            return cuda_fail(ctx, e, "cudaMalloc(attention scratch of a capture)");
+        }
+    }
+    blocks.push_back(b);
+    // kernels leave the counters at zero; in a capture this is a node before them
+    PRISM_CUDA_TRY(ctx, cudaMemsetAsync(b.mem + part_bytes, 0, counts * 4, ctx->stream));
+    *part = reinterpret_cast<float *>(b.mem);
+    *count = reinterpret_cast<unsigned int *>(b.mem + part_bytes);
+    return PRISM_OK;
+}
+
+template <int KIND, int HD>
+static int launch_rows_kernel(prism_cuda_ctx *ctx, const CacheAttnDev &a, uint32_t max_length) {
+    using C = CrCfg<KIND, HD>;
+    static int resident[PRISM_MAX_DEVICES] = {0};          // blocks of an SM; 0: not asked yet
+    if (!resident[ctx->device]) {
+        PRISM_CUDA_TRY(ctx, cudaFuncSetAttribute(cache_rows_kernel<KIND, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+        int n = 0;
+        PRISM_CUDA_TRY(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, cache_rows_kernel<KIND, HD>, CR_THREADS, C::SMEM));
+        if (n < 1) return fail(ctx, PRISM_E_CUDA, "cache_rows_kernel does not fit an SM");
+        resident[ctx->device] = n;
+    }
+    CrDev d{};
+    d.a = a;
+    d.tiles = (uint32_t)(((uint64_t)a.max_tokens * a.group + CR_ROWS - 1) / CR_ROWS);
+    const uint64_t items = (uint64_t)a.n_entries * a.c.kv_heads * d.tiles, slots = (uint64_t)ctx->sm_count * resident[ctx->device];
+    uint64_t seen = max_length;
+    if (a.window) seen = std::min<uint64_t>(seen, (uint64_t)a.window + a.sinks + 2 * C::TP);
+    const uint64_t most = (seen + C::TP * CR_W - 1) / (C::TP * CR_W);  // parts in which every warp has a tile
+    d.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(most, CR_MAX_SPLIT), slots / items));
+    if (items * d.splits > 0x7FFFFFFFull) return fail(ctx, PRISM_E_ARG, "cache_attention: too many rows");
+    if (d.splits > 1) PRISM_TRY(cache_scratch(ctx, (size_t)(items * d.splits) * (CR_ROWS * HD + 32) * 4, (size_t)items, &d.part, &d.count));
+    launch_pdl(ctx, "cache_rows_kernel", cache_rows_kernel<KIND, HD>, dim3((uint32_t)(items * d.splits)), dim3(CR_THREADS), C::SMEM, d);
+    return after_launch(ctx, "cache_rows_kernel");
 }
 
 template <int KIND>
-static void launch_plain(prism_cuda_ctx *ctx, uint32_t hd, const CacheAttnDev &a) {
-    const dim3 grid((uint32_t)(((uint64_t)a.max_tokens * a.heads + 3) / 4), a.n_entries), block(128);
+static int launch_kind(prism_cuda_ctx *ctx, uint32_t hd, const CacheAttnDev &a, uint32_t max_length) {
     switch (hd) {
-    case 32: return launch_pdl(ctx, "cache_attn_plain_kernel", cache_attn_plain_kernel<KIND, 32>, grid, block, 0, a);
-    case 64: return launch_pdl(ctx, "cache_attn_plain_kernel", cache_attn_plain_kernel<KIND, 64>, grid, block, 0, a);
-    case 128: return launch_pdl(ctx, "cache_attn_plain_kernel", cache_attn_plain_kernel<KIND, 128>, grid, block, 0, a);
-    default: return launch_pdl(ctx, "cache_attn_plain_kernel", cache_attn_plain_kernel<KIND, 256>, grid, block, 0, a);
+    case 32: return launch_rows_kernel<KIND, 32>(ctx, a, max_length);
+    case 64: return launch_rows_kernel<KIND, 64>(ctx, a, max_length);
+    case 128: return launch_rows_kernel<KIND, 128>(ctx, a, max_length);
+    default: return launch_rows_kernel<KIND, 256>(ctx, a, max_length);
     }
 }
 
@@ -70,13 +837,12 @@ static int cache_attention(prism_cuda_ctx *ctx, const prism_cache *c, const pris
     a.tree_words = p->tree_words;
     a.q_pos = p->q_pos;
     switch (kind) {
-    case KV_F16: launch_plain<KV_F16>(ctx, c->head_dim, a); break;
-    case KV_BF16: launch_plain<KV_BF16>(ctx, c->head_dim, a); break;
-    case KV_INT8: launch_plain<KV_INT8>(ctx, c->head_dim, a); break;
-    case KV_E4M3: launch_plain<KV_E4M3>(ctx, c->head_dim, a); break;
-    default: launch_plain<KV_INT4>(ctx, c->head_dim, a); break;
+    case KV_F16: return launch_kind<KV_F16>(ctx, c->head_dim, a, p->max_length);
+    case KV_BF16: return launch_kind<KV_BF16>(ctx, c->head_dim, a, p->max_length);
+    case KV_INT8: return launch_kind<KV_INT8>(ctx, c->head_dim, a, p->max_length);
+    case KV_E4M3: return launch_kind<KV_E4M3>(ctx, c->head_dim, a, p->max_length);
+    default: return launch_kind<KV_INT4>(ctx, c->head_dim, a, p->max_length);
     }
-    return after_launch(ctx, "cache_attn_plain_kernel");
 }
 
 }  // namespace prism

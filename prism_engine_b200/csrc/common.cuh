@@ -63,6 +63,8 @@ namespace prism {
 struct PalettizePool;
 void palettize_pool_free(PalettizePool *pool);
 bool palettize_pool_trim(PalettizePool *pool);  // gives the device buffers back; whether there were any
+struct CacheScratch;
+void cache_scratch_free(CacheScratch *scratch);
 }  // namespace prism
 
 // The opaque context of the C ABI.
@@ -140,6 +142,7 @@ struct prism_cuda_ctx {
     // backend-held KV cache of the MetalBackend-style entry points (prism_cuda_kv_init / kv_append / attention_kv)
     uint16_t *kv_k = nullptr, *kv_v = nullptr;
     uint32_t kv_layers = 0, kv_dim = 0, kv_max_seq = 0;
+    prism::CacheScratch *cache_scratch = nullptr;  // of the attention over caller-owned caches (cache_attn.cu)
     prism::PalettizePool *palettize = nullptr;  // of the quantiser's host entry point (palettize.cu)
     // execution plan of the last .cimage that was loaded (src/lut/graph.rs:552-589); version 0: none / unparseable
     struct PlanInfo {
