@@ -712,7 +712,7 @@ void cache_scratch_free(CacheScratch *s) {
     for (auto &b : s->blocks) cudaFree(b.mem);
     delete s;
 }
-static int cache_scratch(prism_cuda_ctx *ctx, size_t part_bytes, size_t counts, float **part, unsigned int **count) {
+int cache_scratch(prism_cuda_ctx *ctx, size_t part_bytes, size_t counts, float **part, unsigned int **count) {
     if (!ctx->cache_scratch) ctx->cache_scratch = new CacheScratch();
     auto &blocks = ctx->cache_scratch->blocks;
     cudaStreamCaptureStatus status;
@@ -724,7 +724,7 @@ static int cache_scratch(prism_cuda_ctx *ctx, size_t part_bytes, size_t counts, 
         if (b.capture != id) continue;
         if (b.part_bytes >= part_bytes && b.counts >= counts) {
             *part = reinterpret_cast<float *>(b.mem);
-            *count = reinterpret_cast<unsigned int *>(b.mem + b.part_bytes);
+            if (count) *count = reinterpret_cast<unsigned int *>(b.mem + b.part_bytes);
             return PRISM_OK;
         }
         if (id == 0) {
@@ -754,9 +754,9 @@ static int cache_scratch(prism_cuda_ctx *ctx, size_t part_bytes, size_t counts, 
     }
     blocks.push_back(b);
     // kernels leave the counters at zero; in a capture this is a node before them
-    PRISM_CUDA_TRY(ctx, cudaMemsetAsync(b.mem + part_bytes, 0, counts * 4, ctx->stream));
+    if (counts) PRISM_CUDA_TRY(ctx, cudaMemsetAsync(b.mem + part_bytes, 0, counts * 4, ctx->stream));
     *part = reinterpret_cast<float *>(b.mem);
-    *count = reinterpret_cast<unsigned int *>(b.mem + part_bytes);
+    if (count) *count = reinterpret_cast<unsigned int *>(b.mem + part_bytes);
     return PRISM_OK;
 }
 
@@ -836,6 +836,7 @@ static int cache_attention(prism_cuda_ctx *ctx, const prism_cache *c, const pris
     a.tree = p->tree;
     a.tree_words = p->tree_words;
     a.q_pos = p->q_pos;
+    if ((uint64_t)a.max_tokens * a.group > CR_ROWS && cache_tiles_fit(a, c->head_dim)) return launch_cache_tiles(ctx, kind, c->head_dim, a, p->max_length);
     switch (kind) {
     case KV_F16: return launch_kind<KV_F16>(ctx, c->head_dim, a, p->max_length);
     case KV_BF16: return launch_kind<KV_BF16>(ctx, c->head_dim, a, p->max_length);

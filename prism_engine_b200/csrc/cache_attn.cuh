@@ -121,4 +121,10 @@ __device__ __noinline__ void cache_plain_row(const CacheAttnDev &a, const CacheE
 }
 #endif
 
+// Scratch of a call (cache_attn.cu): `part_bytes` and `counts` counters that are zero.
+int cache_scratch(prism_cuda_ctx *ctx, size_t part_bytes, size_t counts, float **part, unsigned int **count);
+// cache_attn_tc5.cu: many rows per cached head; cache_tiles_fit: head size and pool are for it
+bool cache_tiles_fit(const CacheAttnDev &a, uint32_t hd);
+int launch_cache_tiles(prism_cuda_ctx *ctx, int kind, uint32_t hd, const CacheAttnDev &a, uint32_t max_length);
+
 }  // namespace prism
