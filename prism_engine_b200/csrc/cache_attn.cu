@@ -1,51 +1,54 @@
 // Attention of the newest tokens of some sequences over a caller-owned cache (prism_cuda_cache_attention_dev): the kernel for few
 // query rows per cached head.
 //
-// A block takes 16 query rows that share a cached head (the heads of its group, of one token or several) and a part of the
+// A block takes 8 or 16 query rows that share a cached head (the heads of its group, of one token or several) and a part of the
 // positions that any of them sees; its four warps take tiles of 16 or 32 positions in turn, each with its own ring of stages
-// (cp.async), running maximum and sums, so no warp waits for another before the end.  S = q K^T and O += P V are mma.sync with the
-// rows as M.  Codes go from shared memory to fragments in registers, with no 16-bit copy in between: a lane's fragments of K
-// are consecutive codes of a row (the order of a contraction is free, so q's fragments follow it), those of V are the same
-// columns of four rows, their bytes interleaved.  Codes are exact in fp16, so scales stay out of the products:
+// (cp.async), running maximum and sums, so no warp waits for another before the end.  Products are mma.sync with positions, then columns,
+// as M and eight query rows as N: S^T = K q^T, O^T += V^T P^T.  Codes go from shared memory to fragments in registers, with no
+// 16-bit copy in between: a lane's fragments of K are consecutive codes of a row (the order of a contraction is free, so q's
+// fragments follow it), those of V are the same columns of four rows, their bytes interleaved.  Codes are exact in fp16, so scales
+// stay out of the products:
 //   score = (q c) ks + (sum of q) kz,     o = sum of (w vs) c + sum of w vz.
-// w vs enters the product as fp16 over the power of two below the largest vs so far, 2^14-fold, so no scale over- or underflows;
+// w vs enters the product as fp16 over the power of two below the row's largest so far, 2^14-fold, so no scale over- or underflows;
 // with 16-bit rows w itself does (bf16: as it is), and the sum that divides is that of the rounded weights.  q of 8- and 4-bit caches enters
 // as fp16 over a power of two.  Maxima, sums, O and everything that multiplies them are 32 bits.
 //
 // Positions past the end are zero.  A position that some row of the block does not see meets weight 0, which an infinity there turns into
 // NaN: a row whose result is not finite is taken again by itself (cache_plain_row).
 //
-// Where there are fewer rows than SMs the positions are cut into S parts; a block leaves maxima, sums and O in scratch, and the
-// last of a row tile joins them in order.
-// Bound: HBM for long caches, the latency of the chain (places, tiles, joining) for short ones.
+// Where there are fewer row tiles than SMs the positions are cut into S parts, whose maxima, sums and O go to scratch: up to CR_LAST of them
+// the last block to arrive joins in order, more than that cache_join_kernel.
+// Bound: HBM for long caches (with 4-bit codes, the integer instructions of unpacking: some 1.2 a value), the latency of the chain (places,
+// tiles, joining) for short ones.
 #include <algorithm>
 #include <cmath>
 #include <stdexcept>
 #include <vector>
 
-#include "cache_attn.cuh"
+#include "cache_join.cuh"
 
 namespace prism {
 
 constexpr int CR_W = 4, CR_THREADS = CR_W * 32;  // warps of a block
-constexpr uint32_t CR_ROWS = 16, CR_MAX_SPLIT = 256;
+constexpr uint32_t CR_LAST = 16;                 // parts that the last block joins
 constexpr float CR_UP = 16384.0f;                // weights of fp16 products are 2^14-fold
-template <int KIND, int HD>
+template <int KIND, int HD, int NQ>              // NQ: groups of eight query rows
 struct CrCfg {
-    static constexpr int ROWB = HD * (int)kv_bits<KIND>() / 8;
-    static constexpr int TP = ROWB >= 256 ? 16 : 32;                 // positions of a tile
+    static constexpr int ROWB = HD * (int)kv_bits<KIND>() / 8, R = 8 * NQ;
+    static constexpr int TP = ROWB >= 256 ? 16 : 32, MT = TP / 16;   // positions of a tile
     static constexpr int NSC = (int)kv_scales<KIND>();
     static constexpr int TILE = TP * ROWB, SCB = TP * NSC * 4;       // bytes of a tile's keys (or values), of their scales
     static constexpr int STAGE = 2 * TILE + 2 * SCB;
-    static constexpr int ST = ROWB >= 512 ? 2 : ROWB >= 128 ? 3 : 4;
-    static constexpr int KS = HD / 16, CPL = HD / 8;                 // contraction steps of a score; columns of a lane
-    static constexpr bool Q_REGS = HD <= 128;
-    static constexpr int RING = CR_W * ST * STAGE, PARTS = CR_W * (int)CR_ROWS * HD * 4;
-    static constexpr int BODY = RING > PARTS ? RING : PARTS;         // also the warps' parts of O, and the weights of a join
-    static constexpr int Q_OFF = BODY, FRAG_OFF = Q_OFF + (int)CR_ROWS * HD * 2;  // q rows, then as fragments
-    static constexpr int ROW_OFF = FRAG_OFF + HD * 32;               // CrRow of each row, then the warps' maxima and sums
-    static constexpr size_t SMEM = ROW_OFF + 16 * 32 + CR_W * 16 * 8 + 16 * 4 + 16;
-    static_assert(BODY >= (int)(CR_MAX_SPLIT * CR_ROWS * 4), "weights of a join");
+    static constexpr int ST = ROWB >= 64 ? 2 : 3;
+    static constexpr int KS = HD / 16, CPL = HD / 8, OT = HD / 16;   // contraction steps of a score; columns of a lane; tiles of O
+    static constexpr bool Q_REGS = KS * NQ <= 16;
+    static constexpr int PITCH = HD + 4;                             // floats of a row of the joined sums
+    static constexpr int RING = CR_W * ST * STAGE, ACC_OFF = CR_W * R * HD * 4, PARTS = ACC_OFF + R * PITCH * 4;
+    static constexpr int BODY = RING > PARTS ? RING : PARTS;         // also the warps' parts of O and their sum
+    static constexpr int Q_OFF = BODY, FRAG_OFF = Q_OFF + R * HD * 2;  // q rows, then as fragments
+    static constexpr int ROW_OFF = FRAG_OFF + R * HD * 2;            // CrRow of each row, then maxima and sums: the warps', the row's; flags
+    static constexpr size_t SMEM = ROW_OFF + R * 32 + CR_W * R * 8 + R * 8 + (int)CR_LAST * R * 4 + 16;
+    static constexpr int BLOCKS = HD <= 128 && NQ == 1 ? 3 : 2;      // of an SM, for the registers
 };
 struct CrRow {
     const uint64_t *mask;
@@ -58,7 +61,7 @@ static_assert(sizeof(CrRow) == 32, "rows of 32 bytes");
 struct CrDev {
     CacheAttnDev a;
     uint32_t splits, tiles;  // parts of the positions, row tiles of an entry and head
-    float *part;             // [item][split][16 HD + 32]
+    float *part;             // of the blocks (CacheJoinDev)
     unsigned int *count;     // [item], zero between launches
 };
 
@@ -149,10 +152,10 @@ __device__ __forceinline__ float cr_inv_pow2(float p) { return p > 0.0f ? __uint
 
 }  // namespace
 
-template <int KIND, int HD>
-__global__ void __launch_bounds__(CR_THREADS) cache_rows_kernel(const __grid_constant__ CrDev d) {
-    using C = CrCfg<KIND, HD>;
-    constexpr int TP = C::TP, NT = TP / 8, KS = C::KS, CPL = C::CPL, ROWB = C::ROWB, NSC = C::NSC, ST = C::ST;
+template <int KIND, int HD, int NQ>
+__global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache_rows_kernel(const __grid_constant__ CrDev d) {
+    using C = CrCfg<KIND, HD, NQ>;
+    constexpr int TP = C::TP, MT = C::MT, KS = C::KS, CPL = C::CPL, OT = C::OT, ROWB = C::ROWB, NSC = C::NSC, ST = C::ST, R = C::R, PITCH = C::PITCH;
     constexpr bool CODES = KIND >= KV_INT8, BF16 = KIND == KV_BF16;
     const CacheAttnDev &a = d.a;
     extern __shared__ __align__(128) uint8_t cr_smem[];
@@ -163,13 +166,14 @@ __global__ void __launch_bounds__(CR_THREADS) cache_rows_kernel(const __grid_con
     const uint32_t tile = item % d.tiles, kh = item / d.tiles % a.c.kv_heads, e = item / d.tiles / a.c.kv_heads;
     CacheEntry x;
     if (!cache_entry(a, e, x)) return;                     // the same in all blocks of an item
-    const uint32_t n_rows = x.n * a.group, r0 = tile * CR_ROWS;
+    const uint32_t n_rows = x.n * a.group, r0 = tile * R;
     if (r0 >= n_rows) return;
-    const uint32_t here = min(CR_ROWS, n_rows - r0), tok_lo = r0 / a.group, tok_hi = (r0 + here - 1) / a.group;
+    const uint32_t here = min((uint32_t)R, n_rows - r0), tok_lo = r0 / a.group, tok_hi = (r0 + here - 1) / a.group;
 
     CrRow *rows = reinterpret_cast<CrRow *>(cr_smem + C::ROW_OFF);
-    float *w_max = reinterpret_cast<float *>(cr_smem + C::ROW_OFF + 16 * 32), *w_sum = w_max + CR_W * 16, *r_sum = w_sum + CR_W * 16;
-    uint32_t *flags = reinterpret_cast<uint32_t *>(r_sum + 16);  // rows to be taken again; whether this block joins
+    float *w_max = reinterpret_cast<float *>(cr_smem + C::ROW_OFF + R * 32), *w_sum = w_max + CR_W * R, *r_max = w_sum + CR_W * R, *r_sum = r_max + R,
+          *wgt = r_sum + R;
+    uint32_t *flags = reinterpret_cast<uint32_t *>(wgt + CR_LAST * R);  // rows to be taken again; whether this block joins
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(cr_smem) + warp * ST * C::STAGE;
 
     // ---- the positions that some row sees: the first tiles (a.sinks), then main_lo .. ---------------------------------
@@ -231,8 +235,8 @@ __global__ void __launch_bounds__(CR_THREADS) cache_rows_kernel(const __grid_con
 
     // ---- rows and q's fragments -----------------------------------------------------------------------------------------
     {
-        constexpr int PER = HD / 8;                        // values of a thread: eight threads a row
-        const uint32_t r = tid >> 3, part = tid & 7, token = (r0 + r) / a.group;
+        constexpr int TR = CR_THREADS / R, PER = HD / TR;  // threads of a row, values of a thread
+        const uint32_t r = tid / TR, part = tid % TR, token = (r0 + r) / a.group;
         const bool there = r < here;
         uint32_t w[PER / 2];
 #pragma unroll
@@ -242,8 +246,10 @@ __global__ void __launch_bounds__(CR_THREADS) cache_rows_kernel(const __grid_con
             if constexpr (PER >= 8) {
 #pragma unroll
                 for (int i = 0; i < PER / 8; i++) reinterpret_cast<uint4 *>(w)[i] = reinterpret_cast<const uint4 *>(src)[i];
-            } else {
+            } else if constexpr (PER == 4) {
                 *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(src);
+            } else {
+                w[0] = *reinterpret_cast<const uint32_t *>(src);
             }
         }
         float mul = a.scale * 1.4426950408889634f, sum = 0.0f;
@@ -255,7 +261,7 @@ __global__ void __launch_bounds__(CR_THREADS) cache_rows_kernel(const __grid_con
                 big = fmaxf(big, fabsf(v[i]));
             }
 #pragma unroll
-            for (int o = 4; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+            for (int o = TR / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
             const float unit = cr_pow2_below(big), inv = unit > 0.0f ? cr_inv_pow2(unit) : 1.0f;
             if (unit > 0.0f) mul *= unit;
 #pragma unroll
@@ -266,7 +272,7 @@ __global__ void __launch_bounds__(CR_THREADS) cache_rows_kernel(const __grid_con
                 w[i] = *reinterpret_cast<const uint32_t *>(&h);
             }
 #pragma unroll
-            for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+            for (int o = TR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
         }
         uint32_t *dst = reinterpret_cast<uint32_t *>(cr_smem + C::Q_OFF) + (r * HD + part * PER) / 2;
 #pragma unroll
@@ -286,31 +292,46 @@ __global__ void __launch_bounds__(CR_THREADS) cache_rows_kernel(const __grid_con
     __syncthreads();
     {
         const uint16_t *q = reinterpret_cast<const uint16_t *>(cr_smem + C::Q_OFF);
-        uint4 *frag = reinterpret_cast<uint4 *>(cr_smem + C::FRAG_OFF);
-        for (uint32_t s = tid; s < KS * 32; s += CR_THREADS) {
-            const uint32_t ks = s >> 5, ln = s & 31, fg = ln >> 2, ft = ln & 3;
-            uint32_t el[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) el[j] = cr_elem<KIND, HD>(ks, ft, j);
-            auto pair = [&](uint32_t r, int j) { return (uint32_t)q[r * HD + el[j]] | (uint32_t)q[r * HD + el[j + 1]] << 16; };
-            frag[s] = make_uint4(pair(fg, 0), pair(fg + 8, 0), pair(fg, 2), pair(fg + 8, 2));
+        uint2 *frag = reinterpret_cast<uint2 *>(cr_smem + C::FRAG_OFF);
+        for (uint32_t s = tid; s < NQ * KS * 32; s += CR_THREADS) {
+            const uint32_t ks = (s >> 5) % KS, ln = s & 31, fr = (s >> 5) / KS * 8 + (ln >> 2), ft = ln & 3;
+            auto pair = [&](int j) {
+                return (uint32_t)q[fr * HD + cr_elem<KIND, HD>(ks, ft, j)] | (uint32_t)q[fr * HD + cr_elem<KIND, HD>(ks, ft, j + 1)] << 16;
+            };
+            frag[s] = make_uint2(pair(0), pair(2));
         }
     }
     __syncthreads();
-    const uint32_t frag_at = (uint32_t)__cvta_generic_to_shared(cr_smem) + C::FRAG_OFF + lane * 16;
-    uint32_t qf[C::Q_REGS ? KS : 1][4];
+    const uint32_t frag_at = (uint32_t)__cvta_generic_to_shared(cr_smem) + C::FRAG_OFF + lane * 8;
+    uint32_t qf[C::Q_REGS ? NQ * KS : 1][2];
     if constexpr (C::Q_REGS) {
 #pragma unroll
-        for (int k = 0; k < KS; k++) cr_lds<4>(qf[k], frag_at + k * 512);
+        for (int k = 0; k < NQ * KS; k++) cr_lds<2>(qf[k], frag_at + k * 256);
     }
-    const CrRow ra = rows[g], rb = rows[g + 8];
+    float mul[NQ][2], qsum[NQ][2];                         // of the lane's rows 2t and 2t + 1
+#pragma unroll
+    for (int n = 0; n < NQ; n++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            mul[n][h] = rows[n * 8 + 2 * t + h].mul;
+            qsum[n][h] = rows[n * 8 + 2 * t + h].qsum;
+        }
 
     // ---- this warp's tiles ------------------------------------------------------------------------------------------------
-    float o[CPL][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, z[2] = {0.0f, 0.0f}, unit = 0.0f;
+    float o[NQ][OT][4], m[NQ][2], l[NQ][2], z[NQ][2], unit[NQ][2];
 #pragma unroll
-    for (int i = 0; i < CPL; i++)
+    for (int n = 0; n < NQ; n++) {
 #pragma unroll
-        for (int c = 0; c < 4; c++) o[i][c] = 0.0f;
+        for (int h = 0; h < 2; h++) {
+            m[n][h] = -INFINITY;
+            l[n][h] = z[n][h] = 0.0f;
+            unit[n][h] = 0x1p-100f;
+        }
+#pragma unroll
+        for (int i = 0; i < OT; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) o[n][i][c] = 0.0f;
+    }
     uint32_t st = 0;
     for (uint32_t i = i_lo + warp; i < i_hi; i += CR_W) {
         asm volatile("cp.async.wait_group %0;\n" ::"n"(ST - 2) : "memory");
@@ -318,183 +339,200 @@ __global__ void __launch_bounds__(CR_THREADS) cache_rows_kernel(const __grid_con
         fetch(i + (ST - 1) * CR_W, st == 0 ? ST - 1 : st - 1);
         const uint32_t kt = ring + st * C::STAGE, vt = kt + C::TILE, ksc = vt + C::TILE, vsc = ksc + C::SCB;
         const int32_t p0 = pos_of(i);
-        // scores
-        float s[NT][4];
+        // scores: rows g and g + 8 of 16 positions, query rows 2t and 2t + 1
+        float s[MT][NQ][4];
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
+        for (int j = 0; j < MT; j++) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) s[j][c] = 0.0f;
-            const uint32_t r = j * 8 + g;
-            auto step = [&](int k, uint32_t b0, uint32_t b1) {
-                if constexpr (C::Q_REGS) {
-                    cr_mma<BF16>(s[j], qf[k], b0, b1);
-                } else {
-                    uint32_t q4[4];
-                    cr_lds<4>(q4, frag_at + k * 512);
-                    cr_mma<BF16>(s[j], q4, b0, b1);
+            for (int n = 0; n < NQ; n++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) s[j][n][c] = 0.0f;
+            const uint32_t r = j * 16 + g;
+            auto step = [&](int k, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                const uint32_t ka[4] = {a0, a1, a2, a3};
+#pragma unroll
+                for (int n = 0; n < NQ; n++) {
+                    if constexpr (C::Q_REGS) {
+                        cr_mma<BF16>(s[j][n], ka, qf[n * KS + k][0], qf[n * KS + k][1]);
+                    } else {
+                        uint32_t q2[2];
+                        cr_lds<2>(q2, frag_at + (n * KS + k) * 256);
+                        cr_mma<BF16>(s[j][n], ka, q2[0], q2[1]);
+                    }
                 }
             };
             constexpr int LB = ROWB / 4, NW = LB >= 16 ? 4 : LB / 4;  // a lane's bytes of a row, words of an access
 #pragma unroll
             for (int pc = 0; pc < (LB + 15) / 16; pc++) {
-                uint32_t w[NW];
-                if constexpr (LB >= 16) cr_lds<NW>(w, kt + cr_at<ROWB>(r, t + 4 * pc));
-                else if constexpr (LB == 8) cr_lds<NW>(w, kt + cr_at<ROWB>(r, t >> 1) + (t & 1) * 8);
-                else cr_lds<NW>(w, kt + cr_at<ROWB>(r, 0) + t * 4);
+                uint32_t w[2][NW];                         // of rows g and g + 8
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if constexpr (LB >= 16) cr_lds<NW>(w[h], kt + cr_at<ROWB>(r + 8 * h, t + 4 * pc));
+                    else if constexpr (LB == 8) cr_lds<NW>(w[h], kt + cr_at<ROWB>(r + 8 * h, t >> 1) + (t & 1) * 8);
+                    else cr_lds<NW>(w[h], kt + cr_at<ROWB>(r + 8 * h, 0) + t * 4);
+                }
                 if constexpr (KIND <= KV_BF16) {
 #pragma unroll
-                    for (int q = 0; q < NW / 2; q++) step(pc * 2 + q, w[2 * q], w[2 * q + 1]);
+                    for (int q = 0; q < NW / 2; q++) step(pc * 2 + q, w[0][2 * q], w[1][2 * q], w[0][2 * q + 1], w[1][2 * q + 1]);
                 } else if constexpr (KIND == KV_INT4) {
 #pragma unroll
                     for (int q = 0; q < NW; q++) {
-                        uint32_t h[4];
-                        cr_nibbles(w[q], h);
-                        step((pc * 4 + q) * 2, h[0], h[1]);
-                        step((pc * 4 + q) * 2 + 1, h[2], h[3]);
+                        uint32_t h0[4], h1[4];
+                        cr_nibbles(w[0][q], h0);
+                        cr_nibbles(w[1][q], h1);
+                        step((pc * 4 + q) * 2, h0[0], h1[0], h0[1], h1[1]);
+                        step((pc * 4 + q) * 2 + 1, h0[2], h1[2], h0[3], h1[3]);
                     }
                 } else {
 #pragma unroll
                     for (int q = 0; q < NW; q++) {
-                        uint32_t h0, h1;
-                        cr_bytes<KIND>(w[q], h0, h1);
-                        step(pc * 4 + q, h0, h1);
+                        uint32_t h0[2], h1[2];
+                        cr_bytes<KIND>(w[0][q], h0[0], h0[1]);
+                        cr_bytes<KIND>(w[1][q], h1[0], h1[1]);
+                        step(pc * 4 + q, h0[0], h1[0], h0[1], h1[1]);
                     }
                 }
             }
         }
+        float vs[MT][2], vz[MT][2];                        // of the lane's positions
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-            if constexpr (NSC == 2) {
-                uint32_t w[4];
-                cr_lds<4>(w, ksc + (j * 8 + 2 * t) * 8);
+        for (int j = 0; j < MT; j++) {
+            float ks[2], kz[2];
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const float sc = __uint_as_float(w[(c & 1) * 2]), zero = __uint_as_float(w[(c & 1) * 2 + 1]);
-                    s[j][c] = fmaf(s[j][c], sc, (c < 2 ? ra.qsum : rb.qsum) * zero);
+            for (int h = 0; h < 2; h++) {
+                const uint32_t at = (j * 16 + g + 8 * h) * 4 * NSC;
+                if constexpr (NSC == 2) {
+                    uint32_t w[2];
+                    cr_lds<2>(w, ksc + at);
+                    ks[h] = __uint_as_float(w[0]);
+                    kz[h] = __uint_as_float(w[1]);
+                    cr_lds<2>(w, vsc + at);
+                    vs[j][h] = __uint_as_float(w[0]);
+                    vz[j][h] = __uint_as_float(w[1]);
+                } else if constexpr (NSC == 1) {
+                    uint32_t w[1];
+                    cr_lds<1>(w, ksc + at);
+                    ks[h] = __uint_as_float(w[0]);
+                    cr_lds<1>(w, vsc + at);
+                    vs[j][h] = __uint_as_float(w[0]);
                 }
-            } else if constexpr (NSC == 1) {
-                uint32_t w[2];
-                cr_lds<2>(w, ksc + (j * 8 + 2 * t) * 4);
-#pragma unroll
-                for (int c = 0; c < 4; c++) s[j][c] *= __uint_as_float(w[c & 1]);
             }
 #pragma unroll
-            for (int c = 0; c < 4; c++) s[j][c] *= c < 2 ? ra.mul : rb.mul;
+            for (int n = 0; n < NQ; n++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    if constexpr (NSC == 2) s[j][n][c] = fmaf(s[j][n][c], ks[c >> 1], qsum[n][c & 1] * kz[c >> 1]);
+                    else if constexpr (NSC == 1) s[j][n][c] *= ks[c >> 1];
+                    s[j][n][c] *= mul[n][c & 1];
+                }
         }
         const bool whole = p0 + TP - 1 <= all_to && (p0 > low_max || (uint32_t)(p0 + TP) <= a.sinks);
         if (!whole) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const CrRow &r = c < 2 ? ra : rb;
-                uint32_t seen = 0;                         // a bit for each of the lane's columns
-                uint64_t bits = 0;
-                int32_t from = 0;                          // drafted position of bit 0
-                if (a.tree && r.mask && p0 + TP > x.first) {
-                    from = max(p0 - x.first, 0);
-                    bits = __ldg(r.mask + (from >> 6)) >> (from & 63);
-                    if ((from & 63) && (from >> 6) + 1 < (int32_t)a.tree_words) bits |= __ldg(r.mask + (from >> 6) + 1) << (64 - (from & 63));
-                }
+            for (int n = 0; n < NQ; n++)
 #pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    const int32_t p = p0 + j * 8 + 2 * t + (c & 1);
-                    bool see = p <= r.last && (p > r.low || (uint32_t)p < a.sinks);
-                    if (a.tree && p >= x.first) see = r.mask && p < x.len && (bits >> (p - x.first - from) & 1);
-                    seen |= (uint32_t)see << j;
-                }
+                for (int h = 0; h < 2; h++) {
+                    const CrRow r = rows[n * 8 + 2 * t + h];
 #pragma unroll
-                for (int j = 0; j < NT; j++)
-                    if (!(seen >> j & 1)) s[j][c] = -INFINITY;
-            }
+                    for (int j = 0; j < MT; j++)
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            const int32_t p = p0 + j * 16 + g + 8 * c;
+                            bool see = p <= r.last && (p > r.low || (uint32_t)p < a.sinks);
+                            if (a.tree && p >= x.first) {
+                                see = r.mask && p < x.len;
+                                if (see) see = __ldg(r.mask + ((uint32_t)(p - x.first) >> 6)) >> ((p - x.first) & 63) & 1;
+                            }
+                            if (!see) s[j][n][2 * c + h] = -INFINITY;
+                        }
+                }
         }
         // weights
-        float alpha[2];
+        uint32_t pf[MT][NQ][2];                            // P^T: positions 2t, 2t + 1 (and 8 on) of row g
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float top = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
+        for (int n = 0; n < NQ; n++) {
+            float alpha[2];
 #pragma unroll
-            for (int j = 1; j < NT; j++) top = fmaxf(top, fmaxf(s[j][2 * h], s[j][2 * h + 1]));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            top = fmaxf(top, m[h]);
-            float sub = top == -INFINITY ? 0.0f : top;     // nothing but scores of -inf so far: weights 0
-            alpha[h] = cr_ex2(m[h] - sub);
-            m[h] = top;
-            l[h] *= alpha[h];
-            z[h] *= alpha[h];
-            if (KIND == KV_F16) sub -= 14.0f;
+            for (int h = 0; h < 2; h++) {
+                float top = fmaxf(s[0][n][h], s[0][n][2 + h]);
+                if constexpr (MT == 2) top = fmaxf(top, fmaxf(s[1][n][h], s[1][n][2 + h]));
 #pragma unroll
-            for (int j = 0; j < NT; j++)
+                for (int q = 4; q < 32; q <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, q));
+                top = fmaxf(top, m[n][h]);
+                float sub = top == -INFINITY ? 0.0f : top;  // nothing but scores of -inf so far: weights 0
+                alpha[h] = cr_ex2(m[n][h] - sub);
+                m[n][h] = top;
+                l[n][h] *= alpha[h];
+                if constexpr (NSC == 2) z[n][h] *= alpha[h];
+                if (KIND == KV_F16) sub -= 14.0f;
 #pragma unroll
-                for (int c = 0; c < 2; c++) s[j][2 * h + c] = cr_ex2(s[j][2 * h + c] - sub);
-        }
-        uint32_t pf[NT][2];                                // rows g and g + 8, columns 2t and 2t + 1 of each 8
-        if constexpr (CODES) {
-            float vs[NT][2], vz[NT][2], top = 0.0f;
+                for (int j = 0; j < MT; j++) {
+                    s[j][n][h] = cr_ex2(s[j][n][h] - sub);
+                    s[j][n][2 + h] = cr_ex2(s[j][n][2 + h] - sub);
+                }
+                if constexpr (CODES) {
+                    float big = 0.0f;
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-                if constexpr (NSC == 2) {
-                    uint32_t w[4];
-                    cr_lds<4>(w, vsc + (j * 8 + 2 * t) * 8);
-#pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        vs[j][c] = __uint_as_float(w[2 * c]);
-                        vz[j][c] = __uint_as_float(w[2 * c + 1]);
+                    for (int j = 0; j < MT; j++) {
+                        l[n][h] += s[j][n][h] + s[j][n][2 + h];
+                        if constexpr (NSC == 2) z[n][h] = fmaf(s[j][n][h], vz[j][0], fmaf(s[j][n][2 + h], vz[j][1], z[n][h]));
+                        s[j][n][h] *= vs[j][0];
+                        s[j][n][2 + h] *= vs[j][1];
+                        big = fmaxf(big, fmaxf(fabsf(s[j][n][h]), fabsf(s[j][n][2 + h])));
                     }
-                } else {
-                    uint32_t w[2];
-                    cr_lds<2>(w, vsc + (j * 8 + 2 * t) * 4);
 #pragma unroll
-                    for (int c = 0; c < 2; c++) vs[j][c] = __uint_as_float(w[c]);
-                }
-                top = fmaxf(top, fmaxf(fabsf(vs[j][0]), fabsf(vs[j][1])));
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            const float next = fmaxf(unit, cr_pow2_below(top)), inv = cr_inv_pow2(next), f = unit * inv;  // next > 0 unless all scales were 0
-            if (next != unit) {
-                alpha[0] *= f;
-                alpha[1] *= f;
-                unit = next;
-            }
+                    for (int q = 4; q < 32; q <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, q));
+                    // what O is over: moved down with the weights so far, up when a product is twice as large
+                    float u = alpha[h] == 1.0f ? unit[n][h] : fmaxf(cr_pow2_below(unit[n][h] * alpha[h]), 0x1p-100f);
+                    if (big >= 2.0f * u) u = cr_pow2_below(big);
+                    const float inv = cr_inv_pow2(u);
+                    alpha[h] = alpha[h] * unit[n][h] * inv;
+                    unit[n][h] = u;
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    l[h] += s[j][2 * h] + s[j][2 * h + 1];
-                    if constexpr (NSC == 2) z[h] = fmaf(s[j][2 * h], vz[j][0], fmaf(s[j][2 * h + 1], vz[j][1], z[h]));
-                    const __half2 p = __floats2half2_rn(s[j][2 * h] * (vs[j][0] * inv * CR_UP), s[j][2 * h + 1] * (vs[j][1] * inv * CR_UP));
-                    pf[j][h] = *reinterpret_cast<const uint32_t *>(&p);
+                    for (int j = 0; j < MT; j++) {
+                        s[j][n][h] *= inv * CR_UP;
+                        s[j][n][2 + h] *= inv * CR_UP;
+                    }
                 }
             }
-        } else {
 #pragma unroll
-            for (int j = 0; j < NT; j++)
+            for (int j = 0; j < MT; j++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int h = 0; h < 2; h++) {              // positions g, g + 8
+                    uint32_t p;
                     if constexpr (BF16) {
-                        const __nv_bfloat162 p = __floats2bfloat162_rn(s[j][2 * h], s[j][2 * h + 1]);
-                        pf[j][h] = *reinterpret_cast<const uint32_t *>(&p);
-                        l[h] += __uint_as_float(pf[j][h] << 16) + __uint_as_float(pf[j][h] & 0xFFFF0000u);
+                        const __nv_bfloat162 b = __floats2bfloat162_rn(s[j][n][2 * h], s[j][n][2 * h + 1]);
+                        p = *reinterpret_cast<const uint32_t *>(&b);
+                        l[n][0] += __uint_as_float(p << 16);
+                        l[n][1] += __uint_as_float(p & 0xFFFF0000u);
                     } else {
-                        const __half2 p = __floats2half2_rn(s[j][2 * h], s[j][2 * h + 1]);
-                        pf[j][h] = *reinterpret_cast<const uint32_t *>(&p);
-                        const float2 b = __half22float2(p);
-                        l[h] += b.x + b.y;
+                        const __half2 b = __floats2half2_rn(s[j][n][2 * h], s[j][n][2 * h + 1]);
+                        p = *reinterpret_cast<const uint32_t *>(&b);
+                        if constexpr (!CODES) {
+                            const float2 f = __half22float2(b);
+                            l[n][0] += f.x;
+                            l[n][1] += f.y;
+                        }
                     }
+                    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(pf[j][n][h]) : "r"(p));
                 }
+            if (__any_sync(0xFFFFFFFFu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+                for (int c = 0; c < OT; c++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) o[n][c][q] *= alpha[q & 1];
+            }
         }
-        if (__any_sync(0xFFFFFFFFu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+        // O^T += V^T P^T, 16 positions at a time: tile c of O is columns 2c and 2c + 1 of every lane's CPL
 #pragma unroll
-            for (int c = 0; c < CPL; c++)
-#pragma unroll
-                for (int q = 0; q < 4; q++) o[c][q] *= alpha[q >> 1];
-        }
-        // O += P V, 16 positions at a time
-#pragma unroll
-        for (int kk = 0; kk < TP / 16; kk++) {
-            const uint32_t pa[4] = {pf[2 * kk][0], pf[2 * kk][1], pf[2 * kk + 1][0], pf[2 * kk + 1][1]};
+        for (int kk = 0; kk < MT; kk++) {
             const uint32_t r[4] = {kk * 16 + 2 * t, kk * 16 + 2 * t + 1, kk * 16 + 2 * t + 8, kk * 16 + 2 * t + 9};
             constexpr int CB = ROWB / 8, NW = CB >= 16 ? 4 : CB >= 4 ? CB / 4 : 1;  // a lane's bytes of a row, words of an access
+            auto step = [&](int c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                const uint32_t va[4] = {a0, a1, a2, a3};
+#pragma unroll
+                for (int n = 0; n < NQ; n++) cr_mma<BF16>(o[n][c], va, pf[kk][n][0], pf[kk][n][1]);
+            };
 #pragma unroll
             for (int pc = 0; pc < (CB + 15) / 16; pc++) {
                 uint32_t w[4][NW];
@@ -508,28 +546,25 @@ __global__ void __launch_bounds__(CR_THREADS) cache_rows_kernel(const __grid_con
 #pragma unroll
                 for (int v = 0; v < NW; v++) {
                     if constexpr (KIND <= KV_BF16) {
-                        const int c = (pc * 4 + v) * 2;
-                        cr_mma<BF16>(o[c], pa, __byte_perm(w[0][v], w[1][v], 0x5410), __byte_perm(w[2][v], w[3][v], 0x5410));
-                        cr_mma<BF16>(o[c + 1], pa, __byte_perm(w[0][v], w[1][v], 0x7632), __byte_perm(w[2][v], w[3][v], 0x7632));
+                        step(pc * 4 + v, __byte_perm(w[0][v], w[1][v], 0x5410), __byte_perm(w[0][v], w[1][v], 0x7632), __byte_perm(w[2][v], w[3][v], 0x5410),
+                             __byte_perm(w[2][v], w[3][v], 0x7632));
                     } else if constexpr (KIND == KV_INT4) {
 #pragma unroll
                         for (int half = 0; half < (CB == 2 ? 1 : 2); half++) {
-                            const int c = (pc * 4 + v) * 8 + half * 4;
+                            const int c = (pc * 4 + v) * 4 + half * 2;
                             uint32_t b0[4], b1[4];
                             cr_nibbles(__byte_perm(w[0][v], w[1][v], half ? 0x7632 : 0x5410), b0);
                             cr_nibbles(__byte_perm(w[2][v], w[3][v], half ? 0x7632 : 0x5410), b1);
-#pragma unroll
-                            for (int q = 0; q < 4; q++) cr_mma<false>(o[c + q], pa, b0[q], b1[q]);
+                            step(c, b0[0], b0[1], b1[0], b1[1]);
+                            step(c + 1, b0[2], b0[3], b1[2], b1[3]);
                         }
                     } else {
 #pragma unroll
                         for (int half = 0; half < 2; half++) {
-                            const int c = (pc * 4 + v) * 4 + half * 2;
                             uint32_t b0[2], b1[2];
                             cr_bytes<KIND>(__byte_perm(w[0][v], w[1][v], half ? 0x7362 : 0x5140), b0[0], b0[1]);
                             cr_bytes<KIND>(__byte_perm(w[2][v], w[3][v], half ? 0x7362 : 0x5140), b1[0], b1[1]);
-#pragma unroll
-                            for (int q = 0; q < 2; q++) cr_mma<false>(o[c + q], pa, b0[q], b1[q]);
+                            step((pc * 4 + v) * 2 + half, b0[0], b0[1], b1[0], b1[1]);
                         }
                     }
                 }
@@ -539,76 +574,68 @@ __global__ void __launch_bounds__(CR_THREADS) cache_rows_kernel(const __grid_con
     }
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");
 
-    // ---- the warps' parts, in the order of fragments: value [column][4][lane] -----------------------------------------------
+    // ---- the warps' parts, in the order of fragments -------------------------------------------------------------------------
     __syncthreads();                                       // the rings are free
-    float *parts = reinterpret_cast<float *>(cr_smem), *sum_of = parts;  // the first warp's place takes the sum
-    constexpr uint32_t VALUES = CR_ROWS * HD;
+    float *parts = reinterpret_cast<float *>(cr_smem), *acc = reinterpret_cast<float *>(cr_smem + C::ACC_OFF);  // [warp][row group, tile][4][lane]; [R][PITCH]
+    constexpr uint32_t VALUES = R * HD;
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
-        if constexpr (NSC == 2) {
-            z[h] += __shfl_xor_sync(0xFFFFFFFFu, z[h], 1);
-            z[h] += __shfl_xor_sync(0xFFFFFFFFu, z[h], 2);
-        }
-        if (t == 0) {
-            w_max[warp * 16 + g + 8 * h] = m[h];
-            w_sum[warp * 16 + g + 8 * h] = l[h];
-        }
-    }
-#pragma unroll
-    for (int c = 0; c < CPL; c++)
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            float v = o[c][q];
-            if constexpr (CODES) v = v * (1.0f / CR_UP) * unit;
-            if constexpr (NSC == 2) v += z[q >> 1];
-            parts[warp * VALUES + (c * 4 + q) * 32 + lane] = v;
-        }
-    __syncthreads();
-    {
-        const uint32_t used = min((uint32_t)CR_W, i_hi - i_lo);  // warps that had a tile
-        float top[2], f[CR_W][2], sum[2] = {0.0f, 0.0f};
+    for (int n = 0; n < NQ; n++) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            top[h] = -INFINITY;
-            for (int w = 0; w < CR_W; w++) top[h] = fmaxf(top[h], w_max[w * 16 + g + 8 * h]);
-            const float sub = top[h] == -INFINITY ? 0.0f : top[h];
 #pragma unroll
-            for (int w = 0; w < CR_W; w++) {
-                f[w][h] = cr_ex2(w_max[w * 16 + g + 8 * h] - sub);
-                sum[h] += w_sum[w * 16 + g + 8 * h] * f[w][h];
+            for (int q = 4; q < 32; q <<= 1) {
+                l[n][h] += __shfl_xor_sync(0xFFFFFFFFu, l[n][h], q);
+                if constexpr (NSC == 2) z[n][h] += __shfl_xor_sync(0xFFFFFFFFu, z[n][h], q);
+            }
+            if (g == 0) {
+                w_max[warp * R + n * 8 + 2 * t + h] = m[n][h];
+                w_sum[warp * R + n * 8 + 2 * t + h] = l[n][h];
             }
         }
-        __syncthreads();
-        if (warp == 0 && t == 0) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                w_max[g + 8 * h] = top[h];
-                r_sum[g + 8 * h] = sum[h];
+        for (int c = 0; c < OT; c++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                float v = o[n][c][q];
+                if constexpr (CODES) v = v * (1.0f / CR_UP) * unit[n][q & 1];
+                if constexpr (NSC == 2) v += z[n][q & 1];
+                parts[warp * VALUES + ((n * OT + c) * 4 + q) * 32 + lane] = v;
             }
+    }
+    __syncthreads();
+    if (tid < R) {
+        float top = -INFINITY, sum = 0.0f;
+        for (int w = 0; w < CR_W; w++) top = fmaxf(top, w_max[w * R + tid]);
+        const float sub = top == -INFINITY ? 0.0f : top;
+        for (int w = 0; w < CR_W; w++) {
+            const float f = cr_ex2(w_max[w * R + tid] - sub);
+            sum += w_sum[w * R + tid] * f;
+            w_max[w * R + tid] = f;                        // from here on: the warp's weight
         }
-        for (uint32_t b = warp; b < (uint32_t)CPL * 4; b += CR_W) {
-            const uint32_t h = b >> 1 & 1;
-            float v = 0.0f;
+        r_max[tid] = top;
+        r_sum[tid] = sum;
+    }
+    __syncthreads();
+    for (uint32_t b = warp; b < (uint32_t)NQ * OT * 4; b += CR_W) {
+        const uint32_t q = b & 3, c = (b >> 2) % OT, row = (b >> 2) / OT * 8 + 2 * t + (q & 1);
+        float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < CR_W; w++)
-                if ((uint32_t)w < used) v += parts[w * VALUES + b * 32 + lane] * (h ? f[w][1] : f[w][0]);
-            sum_of[b * 32 + lane] = v;                     // read by this thread only, before
-        }
+        for (int w = 0; w < CR_W; w++) v += parts[w * VALUES + b * 32 + lane] * w_max[w * R + row];
+        acc[row * PITCH + g * CPL + 2 * c + (q >> 1)] = v;
     }
     __syncthreads();
 
     // ---- the blocks' parts ---------------------------------------------------------------------------------------------------
     if (d.splits > 1) {
-        float *mine = d.part + (size_t)blockIdx.x * (VALUES + 32);
-        const uint32_t live = here > 8 ? 4 : 2;            // fragments of rows 8.. only where there are any
+        constexpr size_t PART = cache_part_floats(R, HD);
+        float *mine = d.part + (size_t)blockIdx.x * PART;
         for (uint32_t i = tid; i < VALUES / 4; i += CR_THREADS)
-            if ((i >> 3 & 3) < live) __stcg(reinterpret_cast<float4 *>(mine) + i, reinterpret_cast<const float4 *>(sum_of)[i]);
-        if (tid < 16) {
-            __stcg(mine + VALUES + tid, w_max[tid]);
-            __stcg(mine + VALUES + 16 + tid, r_sum[tid]);
+            __stcg(reinterpret_cast<float4 *>(mine) + i, *reinterpret_cast<const float4 *>(acc + i % R * PITCH + i / R * 4));
+        if (tid < R) {
+            __stcg(mine + VALUES + tid, r_max[tid]);
+            __stcg(mine + VALUES + R + tid, r_sum[tid]);
         }
+        if (d.splits > CR_LAST) return;                    // cache_join_kernel follows
         __threadfence();
         __syncthreads();
         if (tid == 0) {
@@ -619,76 +646,51 @@ __global__ void __launch_bounds__(CR_THREADS) cache_rows_kernel(const __grid_con
         __syncthreads();
         if (!flags[1]) return;
         __threadfence();
-        const float *all = d.part + (size_t)item * d.splits * (VALUES + 32);
-        float *wgt = parts;                                // [split][16]
-        {
-            const uint32_t r = tid >> 3, k = tid & 7;
+        const float *all = d.part + (size_t)item * d.splits * PART;
+        if (tid < R) {
             float top = -INFINITY, sum = 0.0f;
-            for (uint32_t s = k; s < d.splits; s += 8) top = fmaxf(top, __ldcg(all + (size_t)s * (VALUES + 32) + VALUES + r));
-#pragma unroll
-            for (int q = 4; q > 0; q >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, q));
+#pragma unroll 8
+            for (uint32_t s = 0; s < d.splits; s++) top = fmaxf(top, __ldcg(all + s * PART + VALUES + tid));
             const float sub = top == -INFINITY ? 0.0f : top;
-            for (uint32_t s = k; s < d.splits; s += 8) {
-                const float *p = all + (size_t)s * (VALUES + 32) + VALUES + r;
-                const float f = cr_ex2(__ldcg(p) - sub);
-                wgt[s * 16 + r] = f;
-                sum += __ldcg(p + 16) * f;
+#pragma unroll 8
+            for (uint32_t s = 0; s < d.splits; s++) {
+                const float f = cr_ex2(__ldcg(all + s * PART + VALUES + tid) - sub);
+                wgt[s * R + tid] = f;
+                sum += __ldcg(all + s * PART + VALUES + R + tid) * f;
             }
-#pragma unroll
-            for (int q = 4; q > 0; q >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, q);
-            if (k == 0) r_sum[r] = sum;
+            r_sum[tid] = sum;
         }
         __syncthreads();
-        constexpr int PER = VALUES / 4 / CR_THREADS > 0 ? VALUES / 4 / CR_THREADS : 1;
-        float4 acc[PER];
-#pragma unroll
-        for (int q = 0; q < PER; q++) acc[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (uint32_t s = 0; s < d.splits; s++) {
-            const float4 *p = reinterpret_cast<const float4 *>(all + (size_t)s * (VALUES + 32));
-#pragma unroll
-            for (int q = 0; q < PER; q++) {
-                const uint32_t i = q * CR_THREADS + tid, row = (i & 7) + (i >> 4 & 1) * 8;  // four lanes of one row
-                if ((i >> 3 & 3) < live) {
-                    const float4 v = __ldcg(p + i);
-                    const float f = wgt[s * 16 + row];
-                    acc[q].x = fmaf(v.x, f, acc[q].x);
-                    acc[q].y = fmaf(v.y, f, acc[q].y);
-                    acc[q].z = fmaf(v.z, f, acc[q].z);
-                    acc[q].w = fmaf(v.w, f, acc[q].w);
-                }
+        for (uint32_t i = tid; i < VALUES / 4; i += CR_THREADS) {
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+            for (uint32_t s = 0; s < d.splits; s++) {
+                const float4 u = __ldcg(reinterpret_cast<const float4 *>(all + s * PART) + i);
+                const float f = wgt[s * R + i % R];
+                v.x = fmaf(u.x, f, v.x);
+                v.y = fmaf(u.y, f, v.y);
+                v.z = fmaf(u.z, f, v.z);
+                v.w = fmaf(u.w, f, v.w);
             }
+            *reinterpret_cast<float4 *>(acc + i % R * PITCH + i / R * 4) = v;
         }
-        __syncthreads();                                   // the weights have been read
-#pragma unroll
-        for (int q = 0; q < PER; q++) reinterpret_cast<float4 *>(sum_of)[q * CR_THREADS + tid] = acc[q];
         __syncthreads();
     }
 
-    // ---- results: eight columns of a row a thread ----------------------------------------------------------------------------
-    constexpr uint32_t COLS = CPL >= 8 ? 8 : 4;            // consecutive columns that a thread stores
-    for (uint32_t u = tid; u < VALUES / COLS; u += CR_THREADS) {
-        const uint32_t ln = u & 31, q = u >> 5 & 3, c0 = (u >> 7) * COLS, r = (ln >> 2) + (q >> 1) * 8;
+    // ---- results: four columns of a row a thread ------------------------------------------------------------------------------
+    for (uint32_t u = tid; u < VALUES / 4; u += CR_THREADS) {
+        const uint32_t r = u / (HD / 4), c = u % (HD / 4) * 4;
         if (r >= here) continue;
         const float sum = r_sum[r], inv = 1.0f / sum;
-        float v[COLS];
-        bool odd = !(sum > 0.0f);
-#pragma unroll
-        for (uint32_t i = 0; i < COLS; i++) {
-            v[i] = sum_of[((c0 + i) * 4 + q) * 32 + ln] * inv;
-            odd |= !isfinite(v[i]);
-        }
-        if (odd) {
+        float4 v = *reinterpret_cast<const float4 *>(acc + r * PITCH + c);
+        v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        if (!(sum > 0.0f) || !isfinite(v.x) || !isfinite(v.y) || !isfinite(v.z) || !isfinite(v.w)) {
             atomicOr(flags, 1u << r);
             continue;
         }
-        const uint32_t rr = r0 + r, col = (2 * (ln & 3) + (q & 1)) * CPL + c0;
-        uint16_t *dst = a.out + (size_t)(x.row0 + rr / a.group) * a.out_stride + (size_t)(kh * a.group + rr % a.group) * HD + col;
-        uint32_t w[COLS / 2];
-#pragma unroll
-        for (uint32_t i = 0; i < COLS / 2; i++) w[i] = kv_round2(v[2 * i], v[2 * i + 1], a.c.rows_bf16);
-        if constexpr (COLS == 8) *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-        else *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+        const uint32_t rr = r0 + r;
+        uint16_t *dst = a.out + (size_t)(x.row0 + rr / a.group) * a.out_stride + (size_t)(kh * a.group + rr % a.group) * HD + c;
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(kv_round2(v.x, v.y, a.c.rows_bf16), kv_round2(v.z, v.w, a.c.rows_bf16));
     }
     __syncthreads();
     const uint32_t again = flags[0];
@@ -760,38 +762,40 @@ int cache_scratch(prism_cuda_ctx *ctx, size_t part_bytes, size_t counts, float *
     return PRISM_OK;
 }
 
-template <int KIND, int HD>
+template <int KIND, int HD, int NQ>
 static int launch_rows_kernel(prism_cuda_ctx *ctx, const CacheAttnDev &a, uint32_t max_length) {
-    using C = CrCfg<KIND, HD>;
+    using C = CrCfg<KIND, HD, NQ>;
     static int resident[PRISM_MAX_DEVICES] = {0};          // blocks of an SM; 0: not asked yet
     if (!resident[ctx->device]) {
-        PRISM_CUDA_TRY(ctx, cudaFuncSetAttribute(cache_rows_kernel<KIND, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+        PRISM_CUDA_TRY(ctx, cudaFuncSetAttribute(cache_rows_kernel<KIND, HD, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
         int n = 0;
-        PRISM_CUDA_TRY(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, cache_rows_kernel<KIND, HD>, CR_THREADS, C::SMEM));
+        PRISM_CUDA_TRY(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, cache_rows_kernel<KIND, HD, NQ>, CR_THREADS, C::SMEM));
         if (n < 1) return fail(ctx, PRISM_E_CUDA, "cache_rows_kernel does not fit an SM");
         resident[ctx->device] = n;
     }
     CrDev d{};
     d.a = a;
-    d.tiles = (uint32_t)(((uint64_t)a.max_tokens * a.group + CR_ROWS - 1) / CR_ROWS);
+    d.tiles = (uint32_t)(((uint64_t)a.max_tokens * a.group + C::R - 1) / C::R);
     const uint64_t items = (uint64_t)a.n_entries * a.c.kv_heads * d.tiles, slots = (uint64_t)ctx->sm_count * resident[ctx->device];
     uint64_t seen = max_length;
     if (a.window) seen = std::min<uint64_t>(seen, (uint64_t)a.window + a.sinks + 2 * C::TP);
     const uint64_t most = (seen + C::TP * CR_W - 1) / (C::TP * CR_W);  // parts in which every warp has a tile
-    d.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(most, CR_MAX_SPLIT), slots / items));
+    d.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(most, CJ_MAX_SPLIT), slots / items));
     if (items * d.splits > 0x7FFFFFFFull) return fail(ctx, PRISM_E_ARG, "cache_attention: too many rows");
-    if (d.splits > 1) PRISM_TRY(cache_scratch(ctx, (size_t)(items * d.splits) * (CR_ROWS * HD + 32) * 4, (size_t)items, &d.part, &d.count));
-    launch_pdl(ctx, "cache_rows_kernel", cache_rows_kernel<KIND, HD>, dim3((uint32_t)(items * d.splits)), dim3(CR_THREADS), C::SMEM, d);
-    return after_launch(ctx, "cache_rows_kernel");
+    if (d.splits > 1) PRISM_TRY(cache_scratch(ctx, (size_t)(items * d.splits) * cache_part_floats(C::R, HD) * 4, (size_t)items, &d.part, &d.count));
+    launch_pdl(ctx, "cache_rows_kernel", cache_rows_kernel<KIND, HD, NQ>, dim3((uint32_t)(items * d.splits)), dim3(CR_THREADS), C::SMEM, d);
+    PRISM_TRY(after_launch(ctx, "cache_rows_kernel"));
+    return d.splits > CR_LAST ? launch_cache_join<KIND, HD>(ctx, CacheJoinDev{a, d.splits, d.tiles, (uint32_t)C::R, d.part}) : PRISM_OK;
 }
 
 template <int KIND>
 static int launch_kind(prism_cuda_ctx *ctx, uint32_t hd, const CacheAttnDev &a, uint32_t max_length) {
+    const bool one = (uint64_t)a.max_tokens * a.group <= 8;
     switch (hd) {
-    case 32: return launch_rows_kernel<KIND, 32>(ctx, a, max_length);
-    case 64: return launch_rows_kernel<KIND, 64>(ctx, a, max_length);
-    case 128: return launch_rows_kernel<KIND, 128>(ctx, a, max_length);
-    default: return launch_rows_kernel<KIND, 256>(ctx, a, max_length);
+    case 32: return one ? launch_rows_kernel<KIND, 32, 1>(ctx, a, max_length) : launch_rows_kernel<KIND, 32, 2>(ctx, a, max_length);
+    case 64: return one ? launch_rows_kernel<KIND, 64, 1>(ctx, a, max_length) : launch_rows_kernel<KIND, 64, 2>(ctx, a, max_length);
+    case 128: return one ? launch_rows_kernel<KIND, 128, 1>(ctx, a, max_length) : launch_rows_kernel<KIND, 128, 2>(ctx, a, max_length);
+    default: return one ? launch_rows_kernel<KIND, 256, 1>(ctx, a, max_length) : launch_rows_kernel<KIND, 256, 2>(ctx, a, max_length);
     }
 }
 
@@ -836,7 +840,7 @@ static int cache_attention(prism_cuda_ctx *ctx, const prism_cache *c, const pris
     a.tree = p->tree;
     a.tree_words = p->tree_words;
     a.q_pos = p->q_pos;
-    if ((uint64_t)a.max_tokens * a.group > CR_ROWS && cache_tiles_fit(a, c->head_dim)) return launch_cache_tiles(ctx, kind, c->head_dim, a, p->max_length);
+    if ((uint64_t)a.max_tokens * a.group > 16 && cache_tiles_fit(a, c->head_dim)) return launch_cache_tiles(ctx, kind, c->head_dim, a, p->max_length);
     switch (kind) {
     case KV_F16: return launch_kind<KV_F16>(ctx, c->head_dim, a, p->max_length);
     case KV_BF16: return launch_kind<KV_BF16>(ctx, c->head_dim, a, p->max_length);

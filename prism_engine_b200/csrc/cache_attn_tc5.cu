@@ -606,33 +606,37 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         }
         uint4 reg[MINE];
         float2 scr[2][2];                                          // keys', values' scales of positions ct and ct + 96
-        uint32_t at_k = 0, at_v = 0;                               // lanes 0..7: the pool row of the tile's 16-position unit
+        uint32_t at_k = 0, at_v = 0;                               // lanes 0..7: the pool row of the tile's 16-position unit (0 where there is none)
         auto units = [&](int32_t p0) {
             uint32_t page;
             const int32_t p = p0 + (int32_t)(lane & 7) * 16;
-            return p < x.len && kv_page(a.c, x.seq, (uint32_t)p, page) ? (uint32_t)kv_row(a.c, page, kh, (uint32_t)p) : 0xFFFFFFFFu;
+            return p < x.len && kv_page(a.c, x.seq, (uint32_t)p, page) ? (uint32_t)kv_row(a.c, page, kh, (uint32_t)p) : 0u;
         };
         // Four pieces at a time, so that what they wait for overlaps.
         constexpr int G = 4;
-        auto load = [&](const uint8_t *pool, int first, int32_t p0, uint32_t of) {
+        auto load = [&](const uint8_t *pool, int first, uint32_t of) {
             uint32_t at[G];
 #pragma unroll
             for (int i = 0; i < G; i++) at[i] = __shfl_sync(0xFFFFFFFFu, of, ((row0 + (first + i) * STEP) >> 4) & 7);
 #pragma unroll
-            for (int i = 0; i < G; i++) {
-                if (first + i >= MINE) continue;
-                const uint32_t row = row0 + (first + i) * STEP;
-                reg[first + i] = make_uint4(0, 0, 0, 0);
-                if (row < CT_POS && at[i] != 0xFFFFFFFFu && p0 + (int32_t)row < x.len)
-                    reg[first + i] = t5::ldg128_nc(pool + (size_t)(at[i] + (row & 15)) * C::ROWB + piece * 16);
+            for (int i = 0; i < G; i++)
+                if (first + i < MINE) reg[first + i] = t5::ldg128_nc(pool + (size_t)(at[i] + ((row0 + (first + i) * STEP) & 15)) * C::ROWB + piece * 16);
+        };
+        // Past the end some row of the pool is read; its scale is 0, but a code of e4m3 may be NaN.
+        auto clear = [&](int32_t p0) {
+            if (KIND == KV_E4M3 && p0 + CT_POS > x.len) {
+#pragma unroll
+                for (int i = 0; i < MINE; i++)
+                    if (p0 + (int32_t)(row0 + i * STEP) >= x.len) reg[i] = make_uint4(0, 0, 0, 0);
             }
         };
+        constexpr int FULL = CT_POS / STEP;                        // pieces that every thread has
         auto load_scales = [&](int32_t p0, uint32_t of) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const uint32_t row = ct + h * 96, at = __shfl_sync(0xFFFFFFFFu, of, (row >> 4) & 7);
                 scr[0][h] = scr[1][h] = make_float2(0.0f, 0.0f);
-                if (row < CT_POS && at != 0xFFFFFFFFu && p0 + (int32_t)row < x.len) {
+                if (row < CT_POS && p0 + (int32_t)row < x.len) {
                     const size_t from = ((size_t)at + (row & 15)) * NSC;
                     if constexpr (NSC == 2) {
                         scr[0][h] = __ldg(reinterpret_cast<const float2 *>(a.c.ks + from));
@@ -647,7 +651,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         if (n) {
             at_k = units(pos_of(0));
 #pragma unroll
-            for (int i = 0; i < MINE; i += G) load(a.c.k, i, pos_of(0), at_k);
+            for (int i = 0; i < MINE; i += G) load(a.c.k, i, at_k);
             load_scales(pos_of(0), at_k);
         }
         for (uint32_t j = 0; j < n; j++) {
@@ -685,36 +689,38 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                     else vsc[row] = sc.x;
                 }
             }
-            at_k = next < x.len ? units(next) : 0xFFFFFFFFu;
+            at_k = next < x.len ? units(next) : 0u;
             load_scales(next, at_k);
             const uint32_t kt = base + C::K_OFF + st * C::TILE, vt = base + C::V_OFF + st * C::TILE;
+            clear(now);
 #pragma unroll
             for (int g = 0; g < MINE; g += G) {
 #pragma unroll
                 for (int i = g; i < g + G && i < MINE; i++)
-                    if (row0 + i * STEP < CT_POS) ct_convert<KIND, false>(kt + i * STEP * 128, STEP % 8 ? (i & 1) << 6 : 0, to, swap, reg[i], make_float2(1.0f, 0.0f));
-                load(a.c.v, g, now, at_v);
+                    if (i < FULL || row0 + i * STEP < CT_POS) ct_convert<KIND, false>(kt + i * STEP * 128, STEP % 8 ? (i & 1) << 6 : 0, to, swap, reg[i], make_float2(1.0f, 0.0f));
+                load(a.c.v, g, at_v);
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             t5::mbar_arrive(b_kfull + 8 * st);
             asm volatile("bar.sync 9, 96;\n" ::: "memory");        // the scales of all three warps
             t5::mbar_wait_warp(b_vempty + 8 * st, ph ^ 1, err_flag);
             const uint32_t v_at = base + C::SC_OFF + (j % CT_SC) * C::SLOT + (CT_POS + row0) * NSC * 4;
+            clear(now);
 #pragma unroll
             for (int g = 0; g < MINE; g += G) {
                 float2 sc[G];
 #pragma unroll
                 for (int i = 0; i < G; i++) {
                     sc[i] = make_float2(0.0f, 0.0f);
-                    if (g + i < MINE && row0 + (g + i) * STEP < CT_POS) {
+                    if (g + i < MINE && (g + i < FULL || row0 + (g + i) * STEP < CT_POS)) {
                         if constexpr (NSC == 2) sc[i] = ct_lds2(v_at + (g + i) * STEP * NSC * 4);
                         else sc[i].x = ct_lds(v_at + (g + i) * STEP * NSC * 4);
                     }
                 }
 #pragma unroll
                 for (int i = g; i < g + G && i < MINE; i++)
-                    if (row0 + i * STEP < CT_POS) ct_convert<KIND, true>(vt + i * STEP * 128, STEP % 8 ? (i & 1) << 6 : 0, to, swap, reg[i], sc[i - g]);
-                load(a.c.k, g, next, at_k);
+                    if (i < FULL || row0 + i * STEP < CT_POS) ct_convert<KIND, true>(vt + i * STEP * 128, STEP % 8 ? (i & 1) << 6 : 0, to, swap, reg[i], sc[i - g]);
+                load(a.c.k, g, at_k);
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             t5::mbar_arrive(b_vfull + 8 * st);

@@ -17,17 +17,18 @@ struct CacheJoinDev {
     const float *part;             // [item][split]
 };
 
-constexpr uint32_t CJ_THREADS = 256, CJ_MAX_SPLIT = 256;
+constexpr uint32_t CJ_THREADS = 256, CJ_ROWS = 8, CJ_MAX_SPLIT = 256;
 
-// A block takes 8, 16 or 32 rows: weights of their parts, then every thread its groups of four columns over all parts in order.  A row
+// A block takes 8 rows: weights of their parts, then every thread its groups of four columns over all parts in order.  A row
 // whose result is not finite is taken again by itself.  Bound: L2, the parts are read where they were just written.
 template <int KIND, int HD>
 __global__ void __launch_bounds__(CJ_THREADS) cache_join_kernel(const __grid_constant__ CacheJoinDev d) {
-    __shared__ float wgt[CJ_MAX_SPLIT][32];
-    __shared__ float sums[32];
+    __shared__ float wgt[CJ_MAX_SPLIT][CJ_ROWS];
+    __shared__ float sums[CJ_ROWS];
     __shared__ uint32_t again;
     const CacheAttnDev &a = d.a;
-    const uint32_t tid = threadIdx.x, R = min(d.rows, 32u), item = blockIdx.y, r0 = blockIdx.x * R;  // R: 8, 16 or 32
+    constexpr uint32_t R = CJ_ROWS;
+    const uint32_t tid = threadIdx.x, item = blockIdx.y, r0 = blockIdx.x * R;
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t tile = item % d.tiles, kh = item / d.tiles % a.c.kv_heads, e = item / d.tiles / a.c.kv_heads;
@@ -39,18 +40,20 @@ __global__ void __launch_bounds__(CJ_THREADS) cache_join_kernel(const __grid_con
     const size_t size = cache_part_floats(d.rows, HD);
     const float *all = d.part + (size_t)item * d.splits * size;
     {
-        const uint32_t per = CJ_THREADS / R, r = tid / per, k = tid % per;  // threads of a row: 8, 16 or 32 of a warp
+        const uint32_t r = tid >> 5, k = tid & 31;                     // a warp a row
         const float *ml = all + (size_t)d.rows * HD + r0 + r;
         float top = -INFINITY, sum = 0.0f;
-        for (uint32_t s = k; s < d.splits; s += per) top = fmaxf(top, __ldcg(ml + s * size));
-        for (uint32_t o = per / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        for (uint32_t s = k; s < d.splits; s += 32) top = fmaxf(top, __ldcg(ml + s * size));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
         const float sub = top == -INFINITY ? 0.0f : top;
-        for (uint32_t s = k; s < d.splits; s += per) {
+        for (uint32_t s = k; s < d.splits; s += 32) {
             const float f = exp2f(__ldcg(ml + s * size) - sub);
             wgt[s][r] = f;
             sum += __ldcg(ml + s * size + d.rows) * f;
         }
-        for (uint32_t o = per / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
         if (k == 0) sums[r] = sum;
         if (tid == 0) again = 0;
     }
@@ -90,7 +93,7 @@ __global__ void __launch_bounds__(CJ_THREADS) cache_join_kernel(const __grid_con
 template <int KIND, int HD>
 inline int launch_cache_join(prism_cuda_ctx *ctx, const CacheJoinDev &d) {
     const uint32_t items = d.a.n_entries * d.a.c.kv_heads * d.tiles;  // fewer than the GPU has room for: at most 65535
-    launch_pdl(ctx, "cache_join_kernel", cache_join_kernel<KIND, HD>, dim3((d.rows + 31) / 32, items), dim3(CJ_THREADS), 0, d);
+    launch_pdl(ctx, "cache_join_kernel", cache_join_kernel<KIND, HD>, dim3((d.rows + CJ_ROWS - 1) / CJ_ROWS, items), dim3(CJ_THREADS), 0, d);
     return after_launch(ctx, "cache_join_kernel");
 }
 

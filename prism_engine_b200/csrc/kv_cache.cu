@@ -8,9 +8,10 @@
 // Every step is one rounded 32-bit operation, so codes and scales are the same numbers wherever they are computed.  A span below
 // 2^-100 (its reciprocal would overflow) is written with scale 0; a head with a value that is not finite gets the scale NaN.
 //
-// A head of one position is a unit of hd / 8 lanes with 16 bytes of the row each: its extremes take log2(hd / 8) shuffles, and
-// loads and stores of neighbouring heads are whole lines.  Bound: HBM for long lists, launch latency for a decode step's rows; a
-// thread has KV_UNITS units in flight.
+// hd / 16 lanes share a head of a position (a unit), 8 values from each half of it a lane, so loads and stores are whole lines and the extremes take
+// log2(hd / 16) shuffles; a task is four units of one row, so its place is looked up once for them.  Codes are rounded by adding 1.5 * 2^23,
+// whose last bits they then are, and gathered by byte permutes.  Bound: HBM for long lists (the dependent look-ups of place and page in front
+// of a task's data, and the instructions of the divisions, are what is left of it), launch latency for a decode step's rows.
 #include <stdexcept>
 
 #include "kv_cache.cuh"
@@ -24,7 +25,7 @@ struct KvRowsDev {
     uint16_t *k, *v;             // rows, k_stride / v_stride values apart
     uint64_t k_stride, v_stride;
     const int32_t *seq, *pos;    // place of every row
-    uint32_t units;              // n_rows * 2 * kv_heads
+    uint32_t tasks, per_row;     // of all rows, of one: KV_UNITS of its 2 * kv_heads units each
 };
 
 namespace {
@@ -41,29 +42,57 @@ __device__ __forceinline__ uint32_t kv_umax_of(uint32_t v) {
     for (int x = LANES / 2; x > 0; x >>= 1) v = max(v, __shfl_xor_sync(0xFFFFFFFFu, v, x));
     return v;
 }
-
-// Unit u of a list: its row, which of k and v, and its head.
-__device__ __forceinline__ void kv_unit(uint32_t u, uint32_t heads, uint32_t &row, uint32_t &which, uint32_t &head) {
-    const uint32_t t = u / heads;
-    head = u - t * heads;
-    which = t & 1;
-    row = t >> 1;
+template <bool BF16>
+__device__ __forceinline__ void kv_unpack(const uint4 &w, float *x) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (BF16) {
+            x[2 * i] = __uint_as_float(u[i] << 16);
+            x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+}
+template <bool BF16>
+__device__ __forceinline__ uint4 kv_pack(const float *x) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (BF16) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            u[i] = *reinterpret_cast<const uint32_t *>(&h);
+        } else {
+            const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+            u[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+}
+// A rounded number of at most 22 bits (ties to even) in the last bits.
+__device__ __forceinline__ uint32_t kv_rint(float x) { return __float_as_uint(__fadd_rn(x, 12582912.0f)); }
+__device__ __forceinline__ uint32_t kv_four(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {  // their low bytes
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// Codes of 8 values of a head that LANES lanes share, and the head's scales (the same in all its lanes).
+// Codes of 2 * 8 values of a head that LANES lanes share (w[0], w[1]: the first eight, w[2], w[3]: the others; 4-bit codes: w[0] and w[2]),
+// and the head's scales (the same in all its lanes).
 template <int KIND, int LANES>
-__device__ __forceinline__ uint2 kv_encode(const float (&x)[8], float &scale, float &zero) {
+__device__ __forceinline__ void kv_encode(const float (&x)[16], uint32_t (&w)[4], float &scale, float &zero) {
     constexpr float TOP = KIND == KV_INT8 ? 127.0f : KIND == KV_E4M3 ? 448.0f : 15.0f;
     uint32_t big = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) big = max(big, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    for (int i = 0; i < 16; i++) big = max(big, __float_as_uint(x[i]) & 0x7FFFFFFFu);
     big = kv_umax_of<LANES>(big);            // as integers: NaN above infinity above every number
     float lo = 0.0f, span = __uint_as_float(big);
     if (KIND == KV_INT4) {
         float hi = x[0];
         lo = x[0];
 #pragma unroll
-        for (int i = 1; i < 8; i++) {
+        for (int i = 1; i < 16; i++) {
             lo = fminf(lo, x[i]);
             hi = fmaxf(hi, x[i]);
         }
@@ -71,126 +100,174 @@ __device__ __forceinline__ uint2 kv_encode(const float (&x)[8], float &scale, fl
         hi = kv_max_of<LANES>(hi);
         span = __fsub_rn(hi, lo);
     }
-    const bool real = span >= 0x1p-100f, odd = big >= 0x7F800000u || __float_as_uint(span) >= 0x7F800000u;
+    const bool odd = big >= 0x7F800000u || __float_as_uint(span) >= 0x7F800000u, real = span >= 0x1p-100f && !odd;
     scale = real ? __fdiv_rn(span, TOP) : 0.0f;
-    const float inv = real && !odd ? __fdiv_rn(TOP, span) : 0.0f;
+    const float inv = real ? __fdiv_rn(TOP, span) : 0.0f;
     if (KIND == KV_INT4) zero = __fadd_rn(lo, __fmul_rn(8.0f, scale));
     if (odd) scale = zero = __uint_as_float(0x7FC00000u);
-    uint32_t w[2] = {0, 0};
-    if (KIND == KV_INT4) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const float *y = x + 8 * h;
+        w[2 * h] = w[2 * h + 1] = KIND == KV_INT4 ? 0x88888888u : 0;
+        if (KIND == KV_E4M3 ? odd : !real) continue;  // e4m3 keeps the signs of zeros
+        uint32_t c[8];
+        if constexpr (KIND == KV_INT4) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) c[i] = kv_rint(__fmul_rn(__fsub_rn(y[i], lo), inv));
+            uint32_t a = kv_four(c[0], c[1], c[2], c[3]), b = kv_four(c[4], c[5], c[6], c[7]);
+            a |= a >> 4;                     // two codes in bytes 0 and 2
+            b |= b >> 4;
+            w[2 * h] = __byte_perm(a, b, 0x6420);
+        } else if constexpr (KIND == KV_INT8) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) c[i] = kv_rint(__fmul_rn(y[i], inv));
+            w[2 * h] = kv_four(c[0], c[1], c[2], c[3]);
+            w[2 * h + 1] = kv_four(c[4], c[5], c[6], c[7]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) c[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(y[2 * i], inv), __fmul_rn(y[2 * i + 1], inv)), __NV_SATFINITE, __NV_E4M3);
+            w[2 * h] = c[0] | c[1] << 16;
+            w[2 * h + 1] = c[2] | c[3] << 16;
+        }
+    }
+}
+// Eight values of codes: a product in 32 bits, and a sum where there is a zero.
+template <int KIND>
+__device__ __forceinline__ void kv_decode(uint32_t w0, uint32_t w1, float scale, float zero, float *x) {
+    if constexpr (KIND == KV_INT4) {
+#pragma unroll
+        for (int i = 0; i < 8; i++)          // 2^23 + code
+            x[i] = __fadd_rn(__fmul_rn(__uint_as_float((w0 >> (4 * i) & 15u) | 0x4B000000u) - 8388616.0f, scale), zero);
+    } else if constexpr (KIND == KV_INT8) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const int c = real && !odd ? __float2int_rn(__fmul_rn(__fsub_rn(x[i], lo), inv)) : 8;
-            w[0] |= (uint32_t)c << (4 * i);
+            const uint32_t u = (i < 4 ? w0 : w1) ^ 0x80808080u;
+            x[i] = __fmul_rn(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 + (i & 3))) - 8388736.0f, scale);
         }
-    } else if (odd) {
-        // codes 0
-    } else if (KIND == KV_INT8) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) w[i >> 2] |= (uint32_t)(__float2int_rn(__fmul_rn(x[i], inv)) & 0xFF) << (8 * (i & 3));
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            w[i >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(x[2 * i], inv), __fmul_rn(x[2 * i + 1], inv)), __NV_SATFINITE, __NV_E4M3)
-                         << (16 * (i & 1));
+        for (int i = 0; i < 4; i++) {
+            uint32_t h;
+            asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}\n" : "=r"(h) : "r"((i < 2 ? w0 : w1) >> (16 * (i & 1))));
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+            x[2 * i] = __fmul_rn(f.x, scale);
+            x[2 * i + 1] = __fmul_rn(f.y, scale);
+        }
     }
-    return make_uint2(w[0], w[1]);
+}
+
+// A task's row, its place, and its first unit (of 2 * kv_heads: k's heads, then v's).
+struct KvTask {
+    uint32_t row, page, unit;
+    int32_t pos;
+    bool there;
+};
+__device__ __forceinline__ KvTask kv_task(const KvRowsDev &a, uint32_t i) {
+    KvTask t;
+    const uint32_t at = min(i, a.tasks - 1);
+    t.row = at / a.per_row;
+    t.unit = (at - t.row * a.per_row) * KV_UNITS;
+    t.pos = __ldg(a.pos + t.row);
+    t.page = 0;
+    t.there = kv_place(a.c, __ldg(a.seq + t.row), t.pos, t.page) && i < a.tasks;
+    return t;
 }
 
 }  // namespace
 
-template <int KIND, int HD>
-__global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvRowsDev a) {
-    constexpr uint32_t LANES = HD / 8, PER = KV_THREADS / LANES, ROWB = HD * kv_bits<KIND>() / 8;
+template <int KIND, int HD, bool BF16>
+__global__ void __launch_bounds__(KV_THREADS, 3) kv_write_kernel(const KvRowsDev a) {
+    constexpr uint32_t LANES = HD / 16, PER = KV_THREADS / LANES, ROWB = HD * kv_bits<KIND>() / 8;
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t lane = threadIdx.x % LANES, first = blockIdx.x * PER * KV_UNITS + threadIdx.x / LANES;
-    uint4 data[KV_UNITS];
-    size_t to[KV_UNITS];
-    bool there[KV_UNITS];
-    uint32_t which[KV_UNITS];
+    const uint32_t lane = threadIdx.x % LANES, units = 2 * a.c.kv_heads, index = blockIdx.x * PER + threadIdx.x / LANES;
+    const uint32_t row = min(index, a.tasks - 1) / a.per_row, first = (min(index, a.tasks - 1) - row * a.per_row) * KV_UNITS;
+    uint4 data[KV_UNITS][2];                 // asked for before the place is looked up
 #pragma unroll
     for (uint32_t j = 0; j < KV_UNITS; j++) {
-        const uint32_t u = first + j * PER;
-        uint32_t row, head, page = 0;
-        kv_unit(min(u, a.units - 1), a.c.kv_heads, row, which[j], head);
-        const int32_t s = __ldg(a.seq + row), p = __ldg(a.pos + row);
-        data[j] = __ldg(reinterpret_cast<const uint4 *>((which[j] ? a.v + row * a.v_stride : a.k + row * a.k_stride) + head * HD) + lane);
-        there[j] = u < a.units && kv_place(a.c, s, p, page);
-        to[j] = there[j] ? kv_row(a.c, page, head, (uint32_t)p) : 0;
+        const uint32_t u = min(first + j, units - 1), which = u >= a.c.kv_heads, head = u - (which ? a.c.kv_heads : 0);
+        const uint4 *src = reinterpret_cast<const uint4 *>((which ? a.v + row * a.v_stride : a.k + row * a.k_stride) + head * HD);
+        data[j][0] = __ldg(src + lane);
+        data[j][1] = __ldg(src + lane + LANES);
     }
+    const KvTask t = kv_task(a, index);
 #pragma unroll
     for (uint32_t j = 0; j < KV_UNITS; j++) {
-        uint8_t *dst = (which[j] ? a.c.v : a.c.k) + to[j] * ROWB;
+        const uint32_t u = t.unit + j, which = u >= a.c.kv_heads, head = u - (which ? a.c.kv_heads : 0);
+        const bool there = t.there && u < units;
+        const size_t to = there ? kv_row(a.c, t.page, head, (uint32_t)t.pos) : 0;
+        uint8_t *dst = (which ? a.c.v : a.c.k) + to * ROWB;
         if constexpr (KIND <= KV_BF16) {
-            if (there[j]) reinterpret_cast<uint4 *>(dst)[lane] = data[j];
+            if (there) {
+                reinterpret_cast<uint4 *>(dst)[lane] = data[j][0];
+                reinterpret_cast<uint4 *>(dst)[lane + LANES] = data[j][1];
+            }
         } else {
-            float x[8], scale, zero = 0.0f;
-            const uint32_t w[4] = {data[j].x, data[j].y, data[j].z, data[j].w};
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = kv_row_value((uint16_t)(w[i >> 1] >> (16 * (i & 1))), a.c.rows_bf16);
-            const uint2 codes = kv_encode<KIND, LANES>(x, scale, zero);  // every lane of the warp takes part
-            if (!there[j]) continue;
-            float *sc = (which[j] ? a.c.vs : a.c.ks) + to[j] * kv_scales<KIND>();
-            if constexpr (KIND == KV_INT4) {
-                reinterpret_cast<uint32_t *>(dst)[lane] = codes.x;
-                if (lane == 0) *reinterpret_cast<float2 *>(sc) = make_float2(scale, zero);
-            } else {
-                reinterpret_cast<uint2 *>(dst)[lane] = codes;
-                if (lane == 0) *sc = scale;
+            float x[16], scale, zero = 0.0f;
+            uint32_t w[4];
+            kv_unpack<BF16>(data[j][0], x);
+            kv_unpack<BF16>(data[j][1], x + 8);
+            kv_encode<KIND, LANES>(x, w, scale, zero);  // every lane of the warp takes part
+            if (there) {
+                float *sc = (which ? a.c.vs : a.c.ks) + to * kv_scales<KIND>();
+                if constexpr (KIND == KV_INT4) {
+                    reinterpret_cast<uint32_t *>(dst)[lane] = w[0];
+                    reinterpret_cast<uint32_t *>(dst)[lane + LANES] = w[2];
+                    if (lane == 0) *reinterpret_cast<float2 *>(sc) = make_float2(scale, zero);
+                } else {
+                    reinterpret_cast<uint2 *>(dst)[lane] = make_uint2(w[0], w[1]);
+                    reinterpret_cast<uint2 *>(dst)[lane + LANES] = make_uint2(w[2], w[3]);
+                    if (lane == 0) *sc = scale;
+                }
             }
         }
     }
 }
 
-template <int KIND, int HD>
-__global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvRowsDev a) {
-    constexpr uint32_t LANES = HD / 8, PER = KV_THREADS / LANES, ROWB = HD * kv_bits<KIND>() / 8;
+template <int KIND, int HD, bool BF16>
+__global__ void __launch_bounds__(KV_THREADS, 3) kv_read_kernel(const KvRowsDev a) {
+    constexpr uint32_t LANES = HD / 16, PER = KV_THREADS / LANES, ROWB = HD * kv_bits<KIND>() / 8;
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t lane = threadIdx.x % LANES, first = blockIdx.x * PER * KV_UNITS + threadIdx.x / LANES;
-    uint4 data[KV_UNITS];
+    const uint32_t lane = threadIdx.x % LANES, units = 2 * a.c.kv_heads;
+    const KvTask t = kv_task(a, blockIdx.x * PER + threadIdx.x / LANES);
+    if (!t.there) return;
+    uint4 data[KV_UNITS][2];
     float2 sc[KV_UNITS];
-    bool there[KV_UNITS];
 #pragma unroll
     for (uint32_t j = 0; j < KV_UNITS; j++) {
-        const uint32_t u = first + j * PER;
-        uint32_t row, which, head, page = 0;
-        kv_unit(min(u, a.units - 1), a.c.kv_heads, row, which, head);
-        const int32_t s = __ldg(a.seq + row), p = __ldg(a.pos + row);
-        there[j] = u < a.units && kv_place(a.c, s, p, page);
-        data[j] = make_uint4(0, 0, 0, 0);
-        sc[j] = make_float2(0.0f, 0.0f);
-        if (!there[j]) continue;
-        const size_t from = kv_row(a.c, page, head, (uint32_t)p);
+        const uint32_t u = min(t.unit + j, units - 1), which = u >= a.c.kv_heads, head = u - (which ? a.c.kv_heads : 0);
+        const size_t from = kv_row(a.c, t.page, head, (uint32_t)t.pos);
         const uint8_t *src = (which ? a.c.v : a.c.k) + from * ROWB;
         const float *scp = (which ? a.c.vs : a.c.ks) + from * kv_scales<KIND>();
-        if constexpr (KIND <= KV_BF16) data[j] = reinterpret_cast<const uint4 *>(src)[lane];
-        else if constexpr (KIND == KV_INT4) {
-            data[j].x = reinterpret_cast<const uint32_t *>(src)[lane];
-            sc[j] = *reinterpret_cast<const float2 *>(scp);
+        if constexpr (KIND <= KV_BF16) {
+            data[j][0] = __ldg(reinterpret_cast<const uint4 *>(src) + lane);
+            data[j][1] = __ldg(reinterpret_cast<const uint4 *>(src) + lane + LANES);
+        } else if constexpr (KIND == KV_INT4) {
+            data[j][0].x = __ldg(reinterpret_cast<const uint32_t *>(src) + lane);
+            data[j][1].x = __ldg(reinterpret_cast<const uint32_t *>(src) + lane + LANES);
+            sc[j] = __ldg(reinterpret_cast<const float2 *>(scp));
         } else {
-            const uint2 w = reinterpret_cast<const uint2 *>(src)[lane];
-            data[j].x = w.x;
-            data[j].y = w.y;
-            sc[j].x = *scp;
+            const uint2 p = __ldg(reinterpret_cast<const uint2 *>(src) + lane), q = __ldg(reinterpret_cast<const uint2 *>(src) + lane + LANES);
+            data[j][0] = make_uint4(p.x, p.y, 0, 0);
+            data[j][1] = make_uint4(q.x, q.y, 0, 0);
+            sc[j] = make_float2(__ldg(scp), 0.0f);
         }
     }
 #pragma unroll
     for (uint32_t j = 0; j < KV_UNITS; j++) {
-        if (!there[j]) continue;
-        uint32_t row, which, head;
-        kv_unit(first + j * PER, a.c.kv_heads, row, which, head);
-        uint4 *dst = reinterpret_cast<uint4 *>((which ? a.v + row * a.v_stride : a.k + row * a.k_stride) + head * HD) + lane;
-        if constexpr (KIND <= KV_BF16) {
-            *dst = data[j];
-        } else {
-            float x[8];
-            const float both[2] = {sc[j].x, sc[j].y};
-            const uint32_t w[2] = {data[j].x, data[j].y};
-            kv_values<KIND, 8>(reinterpret_cast<const uint8_t *>(w), both, 0, x);
-            *dst = make_uint4(kv_round2(x[0], x[1], a.c.rows_bf16), kv_round2(x[2], x[3], a.c.rows_bf16), kv_round2(x[4], x[5], a.c.rows_bf16),
-                              kv_round2(x[6], x[7], a.c.rows_bf16));
+        const uint32_t u = t.unit + j, which = u >= a.c.kv_heads, head = u - (which ? a.c.kv_heads : 0);
+        if (u >= units) break;
+        uint4 *dst = reinterpret_cast<uint4 *>((which ? a.v + t.row * a.v_stride : a.k + t.row * a.k_stride) + head * HD) + lane;
+#pragma unroll
+        for (uint32_t h = 0; h < 2; h++) {
+            if constexpr (KIND <= KV_BF16) {
+                dst[h * LANES] = data[j][h];
+            } else {
+                float x[8];
+                kv_decode<KIND>(data[j][h].x, data[j][h].y, sc[j].x, sc[j].y, x);
+                dst[h * LANES] = kv_pack<BF16>(x);
+            }
         }
     }
 }
@@ -277,20 +354,25 @@ int kv_check(prism_cuda_ctx *ctx, const prism_cache *c, KvDev *out, int *kind) {
     return PRISM_OK;
 }
 
-template <int KIND>
+template <int KIND, bool BF16>
 static void launch_rows(prism_cuda_ctx *ctx, bool write, uint32_t hd, const KvRowsDev &a) {
-    const uint32_t per = KV_THREADS / (hd / 8) * KV_UNITS;
-    const dim3 grid((a.units + per - 1) / per), block(KV_THREADS);
+    const uint32_t per = KV_THREADS / (hd / 16);
+    const dim3 grid((a.tasks + per - 1) / per), block(KV_THREADS);
     auto go = [&](void (*w)(KvRowsDev), void (*r)(KvRowsDev)) {
         if (write) launch_pdl(ctx, "kv_write_kernel", w, grid, block, 0, a);
         else launch_pdl(ctx, "kv_read_kernel", r, grid, block, 0, a);
     };
     switch (hd) {
-    case 32: return go(kv_write_kernel<KIND, 32>, kv_read_kernel<KIND, 32>);
-    case 64: return go(kv_write_kernel<KIND, 64>, kv_read_kernel<KIND, 64>);
-    case 128: return go(kv_write_kernel<KIND, 128>, kv_read_kernel<KIND, 128>);
-    default: return go(kv_write_kernel<KIND, 256>, kv_read_kernel<KIND, 256>);
+    case 32: return go(kv_write_kernel<KIND, 32, BF16>, kv_read_kernel<KIND, 32, BF16>);
+    case 64: return go(kv_write_kernel<KIND, 64, BF16>, kv_read_kernel<KIND, 64, BF16>);
+    case 128: return go(kv_write_kernel<KIND, 128, BF16>, kv_read_kernel<KIND, 128, BF16>);
+    default: return go(kv_write_kernel<KIND, 256, BF16>, kv_read_kernel<KIND, 256, BF16>);
     }
+}
+template <int KIND>
+static void launch_kind_rows(prism_cuda_ctx *ctx, bool write, uint32_t hd, const KvRowsDev &a) {
+    if (a.c.rows_bf16) launch_rows<KIND, true>(ctx, write, hd, a);
+    else launch_rows<KIND, false>(ctx, write, hd, a);
 }
 
 static int cache_rows(prism_cuda_ctx *ctx, const prism_cache *c, bool write, const void *k, const void *v, uint64_t k_stride, uint64_t v_stride, uint32_t n_rows,
@@ -314,13 +396,14 @@ static int cache_rows(prism_cuda_ctx *ctx, const prism_cache *c, bool write, con
     a.v_stride = v_stride;
     a.seq = seq;
     a.pos = pos;
-    a.units = n_rows * 2 * c->kv_heads;
+    a.per_row = (2 * c->kv_heads + KV_UNITS - 1) / KV_UNITS;
+    a.tasks = n_rows * a.per_row;
     switch (kind) {
     case KV_F16:
-    case KV_BF16: launch_rows<KV_F16>(ctx, write, c->head_dim, a); break;  // 16-bit rows are copied as they are
-    case KV_INT8: launch_rows<KV_INT8>(ctx, write, c->head_dim, a); break;
-    case KV_E4M3: launch_rows<KV_E4M3>(ctx, write, c->head_dim, a); break;
-    default: launch_rows<KV_INT4>(ctx, write, c->head_dim, a); break;
+    case KV_BF16: launch_rows<KV_F16, false>(ctx, write, c->head_dim, a); break;  // 16-bit rows are copied as they are
+    case KV_INT8: launch_kind_rows<KV_INT8>(ctx, write, c->head_dim, a); break;
+    case KV_E4M3: launch_kind_rows<KV_E4M3>(ctx, write, c->head_dim, a); break;
+    default: launch_kind_rows<KV_INT4>(ctx, write, c->head_dim, a); break;
     }
     return after_launch(ctx, write ? "kv_write_kernel" : "kv_read_kernel");
 }
