@@ -10,7 +10,7 @@
 // stay out of the products:
 //   score = (q c) ks + (sum of q) kz,     o = sum of (w vs) c + sum of w vz.
 // w vs enters the product as fp16 over the power of two below the row's largest so far, 2^14-fold, so no scale over- or underflows;
-// with 16-bit rows w itself does (bf16: as it is), and the sum that divides is that of the rounded weights.  q of 8- and 4-bit caches enters
+// with 16-bit rows w itself does (fp16: 2^13-fold, bf16: as it is), and the sum that divides is that of the rounded weights.  q of 8- and 4-bit caches enters
 // as fp16 over a power of two.  Maxima, sums, O and everything that multiplies them are 32 bits.
 //
 // Positions past the end are zero.  A position that some row of the block does not see meets weight 0, which an infinity there turns into
@@ -31,7 +31,8 @@ namespace prism {
 
 constexpr int CR_W = 4, CR_THREADS = CR_W * 32;  // warps of a block
 constexpr uint32_t CR_LAST = 16;                 // parts that the last block joins
-constexpr float CR_UP = 16384.0f;                // weights of fp16 products are 2^14-fold
+constexpr float CR_UP = 16384.0f;                // weights of fp16 products of codes are 2^14-fold, and below 2; of fp16 rows 2^13-fold, and below 2^CR_GROW
+constexpr float CR_GROW = 2.0f;                  // powers of two that a score may lie above the maximum in use
 template <int KIND, int HD, int NQ>              // NQ: groups of eight query rows
 struct CrCfg {
     static constexpr int ROWB = HD * (int)kv_bits<KIND>() / 8, R = 8 * NQ;
@@ -68,9 +69,10 @@ struct CrDev {
 namespace {
 
 // Byte of a 16-byte piece c of tile row r: neighbouring rows' pieces are exchanged so that the lanes that read together (K: four
-// neighbouring pieces of rows 2i and 2i + 1; V: the same columns of rows 0, 2, 4, 6 apart) lie in different banks.
+// neighbouring pieces of rows 2i and 2i + 1; V: the same columns of rows 0, 2, 4, 6 apart) lie in different banks.  Eight rows on it is
+// 8 * ROWB bytes on, and piece c ^ k lies at the place of c with k << 4 exchanged.
 template <int ROWB>
-__device__ __forceinline__ uint32_t cr_at(uint32_t r, uint32_t c) {
+__host__ __device__ constexpr uint32_t cr_at(uint32_t r, uint32_t c) {
     if constexpr (ROWB == 512) return r * 512 + ((c ^ (((r >> 1) & 3) ^ ((r & 1) << 2))) << 4);
     else if constexpr (ROWB == 256) return r * 256 + ((c ^ ((((r >> 1) & 1) | ((r >> 2) & 1) << 2) ^ ((r & 1) << 2))) << 4);
     else if constexpr (ROWB == 128) return r * 128 + ((c ^ (((r >> 1) & 3) << 1 ^ ((r & 1) << 2))) << 4);
@@ -97,11 +99,11 @@ __device__ __forceinline__ float cr_ex2(float x) {
 template <bool BF16>
 __device__ __forceinline__ void cr_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -109,16 +111,22 @@ __device__ __forceinline__ void cr_mma(float (&c)[4], const uint32_t (&a)[4], ui
 __device__ __forceinline__ void cr_cp16(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+// N words of shared memory (plain loads: the compiler takes them early).
 template <int N>
-__device__ __forceinline__ void cr_lds(uint32_t (&w)[N], uint32_t at) {
-    if constexpr (N == 4) asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
-    else if constexpr (N == 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
-    else asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w[0]) : "r"(at) : "memory");
-}
-__device__ __forceinline__ uint32_t cr_lds16(uint32_t at) {
-    uint16_t v;
-    asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(v) : "r"(at) : "memory");
-    return v;
+__device__ __forceinline__ void cr_lds(uint32_t (&w)[N], const uint8_t *p) {
+    if constexpr (N == 4) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        w[0] = v.x;
+        w[1] = v.y;
+        w[2] = v.z;
+        w[3] = v.w;
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        w[0] = v.x;
+        w[1] = v.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t *>(p);
+    }
 }
 __device__ __forceinline__ uint32_t cr_sub2(uint32_t h, uint32_t what) {
     const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&h), *reinterpret_cast<const __half2 *>(&what));
@@ -198,6 +206,17 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
     const uint32_t i_lo = (uint32_t)((uint64_t)n_tiles * split / d.splits), i_hi = (uint32_t)((uint64_t)n_tiles * (split + 1) / d.splits);
     auto pos_of = [&](uint32_t i) { return (int32_t)((i < first_tiles ? i : main_lo + (i - first_tiles)) * TP); };
 
+    // Pages are asked for a tile before its rows, so that no warp waits for the table; pages[u] of 16 positions, the table's own number.
+    uint32_t pages[TP / 16];
+    auto look = [&](uint32_t i) {
+#pragma unroll
+        for (int u = 0; u < TP / 16; u++) {
+            const int32_t p = pos_of(i) + u * 16;
+            pages[u] = 0xFFFFFFFFu;
+            if (i < i_hi && p < x.len) pages[u] = kv_page_number(a.c, x.seq, (uint32_t)p);
+        }
+    };
+    const uint32_t f_at = cr_at<ROWB>(lane / (ROWB / 16), lane % (ROWB / 16));  // of the lane's first piece
     auto fetch = [&](uint32_t i, uint32_t st) {
         if (i < i_hi) {
             const uint32_t kt = ring + st * C::STAGE, vt = kt + C::TILE, ksc = vt + C::TILE, vsc = ksc + C::SCB;
@@ -205,17 +224,18 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
 #pragma unroll
             for (int u = 0; u < TP / 16; u++) {            // a page holds at least 16 positions
                 const int32_t p = p0 + u * 16;
-                uint32_t page = 0;
-                const int32_t left = p < x.len && kv_page(a.c, x.seq, (uint32_t)p, page) ? x.len - p : 0;
-                const size_t row = left ? kv_row(a.c, page, kh, (uint32_t)p) : 0;
-                const uint8_t *ks = a.c.k + row * ROWB, *vs = a.c.v + row * ROWB;
+                const int32_t left = p < x.len && kv_page_ok(a.c, pages[u]) ? x.len - p : 0;
+                const size_t row = left ? kv_row(a.c, pages[u], kh, (uint32_t)p) : 0;
+                const uint8_t *ks = a.c.k + row * ROWB + lane * 16, *vs = a.c.v + row * ROWB + lane * 16;
+                const bool all = left >= 16;
 #pragma unroll
                 for (int m = 0; m < (ROWB + 31) / 32; m++) {
-                    const uint32_t piece = m * 32 + lane, r = piece / (ROWB / 16), c = piece % (ROWB / 16), at = cr_at<ROWB>(u * 16 + r, c);
-                    if (ROWB >= 32 || piece < (uint32_t)ROWB) {
-                        const uint32_t bytes = (int32_t)r < left ? 16 : 0;
-                        cr_cp16(kt + at, ks + piece * 16, bytes);
-                        cr_cp16(vt + at, vs + piece * 16, bytes);
+                    constexpr uint32_t RP = ROWB / 16;
+                    const uint32_t at = (f_at ^ (cr_at<ROWB>(m * 32 / RP, 0) - m * 512)) + u * 16 * ROWB + m * 512;
+                    if (ROWB >= 32 || lane < (uint32_t)ROWB) {
+                        const uint32_t bytes = all || (int32_t)((m * 32 + lane) / RP) < left ? 16 : 0;
+                        cr_cp16(kt + at, ks + m * 512, bytes);
+                        cr_cp16(vt + at, vs + m * 512, bytes);
                     }
                 }
                 if constexpr (NSC > 0) {
@@ -230,8 +250,12 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
         }
         asm volatile("cp.async.commit_group;\n" ::: "memory");
     };
+    look(i_lo + warp);
 #pragma unroll
-    for (int s = 0; s < ST - 1; s++) fetch(i_lo + warp + s * CR_W, s);
+    for (int s = 0; s < ST - 1; s++) {
+        fetch(i_lo + warp + s * CR_W, s);
+        look(i_lo + warp + (s + 1) * CR_W);
+    }
 
     // ---- rows and q's fragments -----------------------------------------------------------------------------------------
     {
@@ -252,7 +276,11 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
                 w[0] = *reinterpret_cast<const uint32_t *>(src);
             }
         }
-        float mul = a.scale * 1.4426950408889634f, sum = 0.0f;
+        float mul = fabsf(a.scale) * 1.4426950408889634f, sum = 0.0f;
+        if (a.scale < 0.0f) {                              // the sign of the scale is q's
+#pragma unroll
+            for (int i = 0; i < PER / 2; i++) w[i] ^= 0x80008000u;
+        }
         if constexpr (CODES) {
             float v[PER], big = 0.0f;
 #pragma unroll
@@ -302,7 +330,7 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
         }
     }
     __syncthreads();
-    const uint32_t frag_at = (uint32_t)__cvta_generic_to_shared(cr_smem) + C::FRAG_OFF + lane * 8;
+    const uint8_t *frag_at = cr_smem + C::FRAG_OFF + lane * 8;
     uint32_t qf[C::Q_REGS ? NQ * KS : 1][2];
     if constexpr (C::Q_REGS) {
 #pragma unroll
@@ -332,67 +360,70 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
 #pragma unroll
             for (int c = 0; c < 4; c++) o[n][i][c] = 0.0f;
     }
+    constexpr int LB = ROWB / 4, CB = ROWB / 8;            // a lane's bytes of a row of keys, of a row of values
+    const uint32_t k_at = LB >= 16 ? cr_at<ROWB>(g, t) : LB == 8 ? cr_at<ROWB>(g, t >> 1) + (t & 1) * 8 : cr_at<ROWB>(g, 0) + t * 4;
+    uint32_t v_at[2];                                      // of rows 2t and 2t + 1
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+        v_at[h] = C::TILE + (CB >= 16 ? cr_at<ROWB>(2 * t + h, g * (CB / 16)) : CB == 8 ? cr_at<ROWB>(2 * t + h, g >> 1) + (g & 1) * 8
+                                        : CB == 4 ? cr_at<ROWB>(2 * t + h, g >> 2) + (g & 3) * 4 : cr_at<ROWB>(2 * t + h, 0) + g * 2);
+    const uint32_t sc_at = 2 * C::TILE + g * 4 * NSC;
     uint32_t st = 0;
     for (uint32_t i = i_lo + warp; i < i_hi; i += CR_W) {
         asm volatile("cp.async.wait_group %0;\n" ::"n"(ST - 2) : "memory");
         __syncwarp();                                      // and the whole warp is done with the tile before
         fetch(i + (ST - 1) * CR_W, st == 0 ? ST - 1 : st - 1);
-        const uint32_t kt = ring + st * C::STAGE, vt = kt + C::TILE, ksc = vt + C::TILE, vsc = ksc + C::SCB;
+        look(i + ST * CR_W);
+        const uint8_t *stage = cr_smem + (warp * ST + st) * C::STAGE;
         const int32_t p0 = pos_of(i);
         // scores: rows g and g + 8 of 16 positions, query rows 2t and 2t + 1
         float s[MT][NQ][4];
 #pragma unroll
-        for (int j = 0; j < MT; j++) {
+        for (int j = 0; j < MT; j++)
 #pragma unroll
             for (int n = 0; n < NQ; n++)
 #pragma unroll
                 for (int c = 0; c < 4; c++) s[j][n][c] = 0.0f;
-            const uint32_t r = j * 16 + g;
-            auto step = [&](int k, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-                const uint32_t ka[4] = {a0, a1, a2, a3};
+        auto step = [&](int j, int k, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+            const uint32_t ka[4] = {a0, a1, a2, a3};
 #pragma unroll
-                for (int n = 0; n < NQ; n++) {
-                    if constexpr (C::Q_REGS) {
-                        cr_mma<BF16>(s[j][n], ka, qf[n * KS + k][0], qf[n * KS + k][1]);
-                    } else {
-                        uint32_t q2[2];
-                        cr_lds<2>(q2, frag_at + (n * KS + k) * 256);
-                        cr_mma<BF16>(s[j][n], ka, q2[0], q2[1]);
-                    }
-                }
-            };
-            constexpr int LB = ROWB / 4, NW = LB >= 16 ? 4 : LB / 4;  // a lane's bytes of a row, words of an access
-#pragma unroll
-            for (int pc = 0; pc < (LB + 15) / 16; pc++) {
-                uint32_t w[2][NW];                         // of rows g and g + 8
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    if constexpr (LB >= 16) cr_lds<NW>(w[h], kt + cr_at<ROWB>(r + 8 * h, t + 4 * pc));
-                    else if constexpr (LB == 8) cr_lds<NW>(w[h], kt + cr_at<ROWB>(r + 8 * h, t >> 1) + (t & 1) * 8);
-                    else cr_lds<NW>(w[h], kt + cr_at<ROWB>(r + 8 * h, 0) + t * 4);
-                }
-                if constexpr (KIND <= KV_BF16) {
-#pragma unroll
-                    for (int q = 0; q < NW / 2; q++) step(pc * 2 + q, w[0][2 * q], w[1][2 * q], w[0][2 * q + 1], w[1][2 * q + 1]);
-                } else if constexpr (KIND == KV_INT4) {
-#pragma unroll
-                    for (int q = 0; q < NW; q++) {
-                        uint32_t h0[4], h1[4];
-                        cr_nibbles(w[0][q], h0);
-                        cr_nibbles(w[1][q], h1);
-                        step((pc * 4 + q) * 2, h0[0], h1[0], h0[1], h1[1]);
-                        step((pc * 4 + q) * 2 + 1, h0[2], h1[2], h0[3], h1[3]);
-                    }
+            for (int n = 0; n < NQ; n++) {
+                if constexpr (C::Q_REGS) {
+                    cr_mma<BF16>(s[j][n], ka, qf[n * KS + k][0], qf[n * KS + k][1]);
                 } else {
-#pragma unroll
-                    for (int q = 0; q < NW; q++) {
-                        uint32_t h0[2], h1[2];
-                        cr_bytes<KIND>(w[0][q], h0[0], h0[1]);
-                        cr_bytes<KIND>(w[1][q], h1[0], h1[1]);
-                        step(pc * 4 + q, h0[0], h1[0], h0[1], h1[1]);
-                    }
+                    uint32_t q2[2];
+                    cr_lds<2>(q2, frag_at + (n * KS + k) * 256);
+                    cr_mma<BF16>(s[j][n], ka, q2[0], q2[1]);
                 }
             }
+        };
+        constexpr int KW = LB >= 16 ? 4 : LB / 4;          // words of an access
+#pragma unroll
+        for (int pc = 0; pc < (LB + 15) / 16; pc++) {
+            uint32_t w[MT][2][KW];                         // of rows g and g + 8 of each 16 positions
+#pragma unroll
+            for (int j = 0; j < MT; j++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) cr_lds<KW>(w[j][h], stage + (k_at ^ (pc * 64)) + (j * 16 + 8 * h) * ROWB);
+#pragma unroll
+            for (int q = 0; q < KW; q++)
+#pragma unroll
+                for (int j = 0; j < MT; j++) {
+                    if constexpr (KIND <= KV_BF16) {
+                        if (q % 2 == 0) step(j, pc * 2 + q / 2, w[j][0][q], w[j][1][q], w[j][0][q + 1], w[j][1][q + 1]);
+                    } else if constexpr (KIND == KV_INT4) {
+                        uint32_t h0[4], h1[4];
+                        cr_nibbles(w[j][0][q], h0);
+                        cr_nibbles(w[j][1][q], h1);
+                        step(j, (pc * 4 + q) * 2, h0[0], h1[0], h0[1], h1[1]);
+                        step(j, (pc * 4 + q) * 2 + 1, h0[2], h1[2], h0[3], h1[3]);
+                    } else {
+                        uint32_t h0[2], h1[2];
+                        cr_bytes<KIND>(w[j][0][q], h0[0], h0[1]);
+                        cr_bytes<KIND>(w[j][1][q], h1[0], h1[1]);
+                        step(j, pc * 4 + q, h0[0], h1[0], h0[1], h1[1]);
+                    }
+                }
         }
         float vs[MT][2], vz[MT][2];                        // of the lane's positions
 #pragma unroll
@@ -400,20 +431,20 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
             float ks[2], kz[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const uint32_t at = (j * 16 + g + 8 * h) * 4 * NSC;
+                const uint8_t *at = stage + sc_at + (j * 16 + 8 * h) * 4 * NSC;
                 if constexpr (NSC == 2) {
                     uint32_t w[2];
-                    cr_lds<2>(w, ksc + at);
+                    cr_lds<2>(w, at);
                     ks[h] = __uint_as_float(w[0]);
                     kz[h] = __uint_as_float(w[1]);
-                    cr_lds<2>(w, vsc + at);
+                    cr_lds<2>(w, at + C::SCB);
                     vs[j][h] = __uint_as_float(w[0]);
                     vz[j][h] = __uint_as_float(w[1]);
                 } else if constexpr (NSC == 1) {
                     uint32_t w[1];
-                    cr_lds<1>(w, ksc + at);
+                    cr_lds<1>(w, at);
                     ks[h] = __uint_as_float(w[0]);
-                    cr_lds<1>(w, vsc + at);
+                    cr_lds<1>(w, at + C::SCB);
                     vs[j][h] = __uint_as_float(w[0]);
                 }
             }
@@ -423,7 +454,6 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
                 for (int c = 0; c < 4; c++) {
                     if constexpr (NSC == 2) s[j][n][c] = fmaf(s[j][n][c], ks[c >> 1], qsum[n][c & 1] * kz[c >> 1]);
                     else if constexpr (NSC == 1) s[j][n][c] *= ks[c >> 1];
-                    s[j][n][c] *= mul[n][c & 1];
                 }
         }
         const bool whole = p0 + TP - 1 <= all_to && (p0 > low_max || (uint32_t)(p0 + TP) <= a.sinks);
@@ -451,47 +481,64 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
         uint32_t pf[MT][NQ][2];                            // P^T: positions 2t, 2t + 1 (and 8 on) of row g
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
-            float alpha[2];
+            // The maximum is moved only when some score of the tile lies above it by more than CR_GROW: else no lane asks the others.
+            float top[2], alpha[2] = {1.0f, 1.0f};
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                float top = fmaxf(s[0][n][h], s[0][n][2 + h]);
-                if constexpr (MT == 2) top = fmaxf(top, fmaxf(s[1][n][h], s[1][n][2 + h]));
+                top[h] = fmaxf(s[0][n][h], s[0][n][2 + h]);
+                if constexpr (MT == 2) top[h] = fmaxf(top[h], fmaxf(s[1][n][h], s[1][n][2 + h]));
+                top[h] = top[h] == -INFINITY ? top[h] : top[h] * mul[n][h];  // mul may be 0
+            }
+            if (__any_sync(0xFFFFFFFFu, top[0] > m[n][0] + CR_GROW || top[1] > m[n][1] + CR_GROW)) {
 #pragma unroll
-                for (int q = 4; q < 32; q <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, q));
-                top = fmaxf(top, m[n][h]);
-                float sub = top == -INFINITY ? 0.0f : top;  // nothing but scores of -inf so far: weights 0
-                alpha[h] = cr_ex2(m[n][h] - sub);
-                m[n][h] = top;
-                l[n][h] *= alpha[h];
-                if constexpr (NSC == 2) z[n][h] *= alpha[h];
-                if (KIND == KV_F16) sub -= 14.0f;
+                for (int h = 0; h < 2; h++) {
 #pragma unroll
-                for (int j = 0; j < MT; j++) {
-                    s[j][n][h] = cr_ex2(s[j][n][h] - sub);
-                    s[j][n][2 + h] = cr_ex2(s[j][n][2 + h] - sub);
+                    for (int q = 4; q < 32; q <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xFFFFFFFFu, top[h], q));
+                    top[h] = fmaxf(top[h], m[n][h]);
+                    alpha[h] = top[h] == -INFINITY ? 1.0f : cr_ex2(m[n][h] - top[h]);
+                    m[n][h] = top[h];
+                    l[n][h] *= alpha[h];
+                    if constexpr (NSC == 2) z[n][h] *= alpha[h];
                 }
-                if constexpr (CODES) {
-                    float big = 0.0f;
+            }
+            float big[2] = {0.0f, 0.0f};
 #pragma unroll
-                    for (int j = 0; j < MT; j++) {
-                        l[n][h] += s[j][n][h] + s[j][n][2 + h];
-                        if constexpr (NSC == 2) z[n][h] = fmaf(s[j][n][h], vz[j][0], fmaf(s[j][n][2 + h], vz[j][1], z[n][h]));
-                        s[j][n][h] *= vs[j][0];
-                        s[j][n][2 + h] *= vs[j][1];
-                        big = fmaxf(big, fmaxf(fabsf(s[j][n][h]), fabsf(s[j][n][2 + h])));
+            for (int h = 0; h < 2; h++) {
+                const float sub = (m[n][h] == -INFINITY ? 0.0f : m[n][h]) - (KIND == KV_F16 ? 13.0f : 0.0f);  // nothing but -inf so far: weights 0
+#pragma unroll
+                for (int j = 0; j < MT; j++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        float &w = s[j][n][2 * c + h];
+                        w = cr_ex2(fmaf(w, mul[n][h], -sub));
+                        if constexpr (CODES) {
+                            l[n][h] += w;
+                            if constexpr (NSC == 2) z[n][h] = fmaf(w, vz[j][c], z[n][h]);
+                            w *= vs[j][c];
+                            big[h] = fmaxf(big[h], fabsf(w));
+                        }
                     }
+            }
+            if constexpr (CODES) {
+                // What O is over: moved down with the weights so far, up when a product is twice as large.
+                if (__any_sync(0xFFFFFFFFu, alpha[0] != 1.0f || alpha[1] != 1.0f || big[0] >= 2.0f * unit[n][0] || big[1] >= 2.0f * unit[n][1])) {
 #pragma unroll
-                    for (int q = 4; q < 32; q <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, q));
-                    // what O is over: moved down with the weights so far, up when a product is twice as large
-                    float u = alpha[h] == 1.0f ? unit[n][h] : fmaxf(cr_pow2_below(unit[n][h] * alpha[h]), 0x1p-100f);
-                    if (big >= 2.0f * u) u = cr_pow2_below(big);
-                    const float inv = cr_inv_pow2(u);
-                    alpha[h] = alpha[h] * unit[n][h] * inv;
-                    unit[n][h] = u;
+                    for (int h = 0; h < 2; h++) {
+#pragma unroll
+                        for (int q = 4; q < 32; q <<= 1) big[h] = fmaxf(big[h], __shfl_xor_sync(0xFFFFFFFFu, big[h], q));
+                        float u = alpha[h] == 1.0f ? unit[n][h] : fmaxf(cr_pow2_below(unit[n][h] * alpha[h]), 0x1p-100f);
+                        if (big[h] >= 2.0f * u) u = cr_pow2_below(big[h]);
+                        alpha[h] = alpha[h] * unit[n][h] * cr_inv_pow2(u);
+                        unit[n][h] = u;
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float inv = cr_inv_pow2(unit[n][h]) * CR_UP;
 #pragma unroll
                     for (int j = 0; j < MT; j++) {
-                        s[j][n][h] *= inv * CR_UP;
-                        s[j][n][2 + h] *= inv * CR_UP;
+                        s[j][n][h] *= inv;
+                        s[j][n][2 + h] *= inv;
                     }
                 }
             }
@@ -526,8 +573,7 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
         // O^T += V^T P^T, 16 positions at a time: tile c of O is columns 2c and 2c + 1 of every lane's CPL
 #pragma unroll
         for (int kk = 0; kk < MT; kk++) {
-            const uint32_t r[4] = {kk * 16 + 2 * t, kk * 16 + 2 * t + 1, kk * 16 + 2 * t + 8, kk * 16 + 2 * t + 9};
-            constexpr int CB = ROWB / 8, NW = CB >= 16 ? 4 : CB >= 4 ? CB / 4 : 1;  // a lane's bytes of a row, words of an access
+            constexpr int NW = CB >= 16 ? 4 : CB >= 4 ? CB / 4 : 1;  // words of an access
             auto step = [&](int c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
                 const uint32_t va[4] = {a0, a1, a2, a3};
 #pragma unroll
@@ -535,13 +581,12 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
             };
 #pragma unroll
             for (int pc = 0; pc < (CB + 15) / 16; pc++) {
-                uint32_t w[4][NW];
+                uint32_t w[4][NW];                         // of rows 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
-                    if constexpr (CB >= 16) cr_lds<NW>(w[q], vt + cr_at<ROWB>(r[q], g * (CB / 16) + pc));
-                    else if constexpr (CB == 8) cr_lds<NW>(w[q], vt + cr_at<ROWB>(r[q], g >> 1) + (g & 1) * 8);
-                    else if constexpr (CB == 4) cr_lds<NW>(w[q], vt + cr_at<ROWB>(r[q], g >> 2) + (g & 3) * 4);
-                    else w[q][0] = cr_lds16(vt + cr_at<ROWB>(r[q], 0) + g * 2);
+                    const uint8_t *at = stage + (v_at[q & 1] ^ (pc * 16)) + (kk * 16 + (q >> 1) * 8) * ROWB;
+                    if constexpr (CB >= 4) cr_lds<NW>(w[q], at);
+                    else w[q][0] = *reinterpret_cast<const uint16_t *>(at);
                 }
 #pragma unroll
                 for (int v = 0; v < NW; v++) {

@@ -563,29 +563,36 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         t5::fence_before();
     } else if constexpr (!CODES) {
         // ================= copies =================
-        if (warp == CT_SOFT && lane == 0) {
-            auto load = [&](const CUtensorMap *map, uint32_t dst, int32_t p0, uint32_t mbar) {
-                t5::mbar_arrive_expect_tx(mbar, CT_POS * HD * 2);
-                for (uint32_t b = 0; b < CT_POS / d.box; b++) {
-                    const int32_t p = p0 + (int32_t)(b * d.box);
-                    uint32_t page = 0, at = d.pool_rows;           // past the last row: zeros
-                    if (p < x.len && kv_page(a.c, x.seq, (uint32_t)p, page)) at = (uint32_t)kv_row(a.c, page, kh, (uint32_t)p);
+        // A lane a box (of at most eight): its page is asked for a tile before it is needed.
+        if (warp == CT_SOFT) {
+            const uint32_t boxes = CT_POS / d.box, b = lane % boxes;
+            auto look = [&](uint32_t j) {
+                const int32_t p = j < n ? pos_of(j) + (int32_t)(b * d.box) : x.len;
+                return p < x.len ? kv_page_number(a.c, x.seq, (uint32_t)p) : 0xFFFFFFFFu;
+            };
+            auto load = [&](const CUtensorMap *map, uint32_t dst, uint32_t at, uint32_t mbar) {
+                if (lane == 0) t5::mbar_arrive_expect_tx(mbar, CT_POS * HD * 2);
+                __syncwarp();
+                if (lane < boxes)
                     for (uint32_t q = 0; q < (uint32_t)C::PANELS; q++)
                         t5::tma_2d(dst + q * C::PANEL + b * d.box * 128, map, (int32_t)(q * 64), (int32_t)at, mbar);
-                }
             };
+            uint32_t page = look(0);
             for (uint32_t j = 0; j < n; j++) {
                 const uint32_t st = j % ST, ph = (j / ST) & 1;
-                const int32_t p0 = pos_of(j);
-                t5::mbar_wait_bounded(b_kempty + 8 * st, ph ^ 1, err_flag);
-                load(&kmap, base + C::K_OFF + st * C::TILE, p0, b_kfull + 8 * st);
-                t5::mbar_wait_bounded(b_vempty + 8 * st, ph ^ 1, err_flag);
-                load(&vmap, base + C::V_OFF + st * C::TILE, p0, b_vfull + 8 * st);
+                const int32_t p = pos_of(j) + (int32_t)(b * d.box);
+                // past the last row of the pool: zeros
+                const uint32_t at = p < x.len && kv_page_ok(a.c, page) ? (uint32_t)kv_row(a.c, page, kh, (uint32_t)p) : d.pool_rows;
+                page = look(j + 1);
+                t5::mbar_wait_warp(b_kempty + 8 * st, ph ^ 1, err_flag);
+                load(&kmap, base + C::K_OFF + st * C::TILE, at, b_kfull + 8 * st);
+                t5::mbar_wait_warp(b_vempty + 8 * st, ph ^ 1, err_flag);
+                load(&vmap, base + C::V_OFF + st * C::TILE, at, b_vfull + 8 * st);
             }
             // every copy in flight lands before the CTA leaves
             for (uint32_t j = n > (uint32_t)ST ? n - ST : 0; j < n; j++) {
-                t5::mbar_wait_bounded(b_kfull + 8 * (j % ST), (j / ST) & 1, err_flag);
-                t5::mbar_wait_bounded(b_vfull + 8 * (j % ST), (j / ST) & 1, err_flag);
+                t5::mbar_wait_warp(b_kfull + 8 * (j % ST), (j / ST) & 1, err_flag);
+                t5::mbar_wait_warp(b_vfull + 8 * (j % ST), (j / ST) & 1, err_flag);
             }
         }
         __syncwarp();
@@ -607,11 +614,16 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         uint4 reg[MINE];
         float2 scr[2][2];                                          // keys', values' scales of positions ct and ct + 96
         uint32_t at_k = 0, at_v = 0;                               // lanes 0..7: the pool row of the tile's 16-position unit (0 where there is none)
-        auto units = [&](int32_t p0) {
-            uint32_t page;
-            const int32_t p = p0 + (int32_t)(lane & 7) * 16;
-            return p < x.len && kv_page(a.c, x.seq, (uint32_t)p, page) ? (uint32_t)kv_row(a.c, page, kh, (uint32_t)p) : 0u;
+        // Pages are asked for two tiles ahead, so that nothing waits for the table.
+        auto look = [&](uint32_t j) {
+            const int32_t p = j < n ? pos_of(j) + (int32_t)(lane & 7) * 16 : x.len;
+            return p < x.len ? kv_page_number(a.c, x.seq, (uint32_t)p) : 0xFFFFFFFFu;
         };
+        auto units = [&](uint32_t j, uint32_t page) {
+            const int32_t p = j < n ? pos_of(j) + (int32_t)(lane & 7) * 16 : x.len;
+            return p < x.len && kv_page_ok(a.c, page) ? (uint32_t)kv_row(a.c, page, kh, (uint32_t)p) : 0u;
+        };
+        uint32_t page = look(0);
         // Four pieces at a time, so that what they wait for overlaps.
         constexpr int G = 4;
         auto load = [&](const uint8_t *pool, int first, uint32_t of) {
@@ -649,7 +661,8 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             }
         };
         if (n) {
-            at_k = units(pos_of(0));
+            at_k = units(0, page);
+            page = look(1);
 #pragma unroll
             for (int i = 0; i < MINE; i += G) load(a.c.k, i, at_k);
             load_scales(pos_of(0), at_k);
@@ -689,7 +702,8 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                     else vsc[row] = sc.x;
                 }
             }
-            at_k = next < x.len ? units(next) : 0u;
+            at_k = units(j + 1, page);
+            page = look(j + 2);
             load_scales(next, at_k);
             const uint32_t kt = base + C::K_OFF + st * C::TILE, vt = base + C::V_OFF + st * C::TILE;
             clear(now);

@@ -31,13 +31,19 @@ struct KvDev {
 #ifdef __CUDACC__
 __device__ __forceinline__ void kv_flag(const KvDev &c) { atomicExch(c.err, 8u); }
 
-// Page of position p of sequence s, both inside the cache's bounds; false (and the error word) where the table names no page of it.
-__device__ __forceinline__ bool kv_page(const KvDev &c, uint32_t s, uint32_t p, uint32_t &page) {
+// Page of position p of sequence s, both inside the cache's bounds, as the table has it; whether it is one (if not, the error word is set).
+__device__ __forceinline__ uint32_t kv_page_number(const KvDev &c, uint32_t s, uint32_t p) {
     const uint32_t at = p >> c.shift;
-    page = c.table ? (uint32_t)__ldg(c.table + (size_t)s * c.stride + at) : s * c.stride + at;
+    return c.table ? (uint32_t)__ldg(c.table + (size_t)s * c.stride + at) : s * c.stride + at;
+}
+__device__ __forceinline__ bool kv_page_ok(const KvDev &c, uint32_t page) {
     if (page < c.n_pages) return true;
     kv_flag(c);
     return false;
+}
+__device__ __forceinline__ bool kv_page(const KvDev &c, uint32_t s, uint32_t p, uint32_t &page) {
+    page = kv_page_number(c, s, p);
+    return kv_page_ok(c, page);
 }
 // Row of a head of a page's position: rows are what codes and scales are counted in.
 __device__ __forceinline__ size_t kv_row(const KvDev &c, uint32_t page, uint32_t head, uint32_t p) {
