@@ -14,7 +14,8 @@
 //
 // Positions past the end are zero.  A position that a row does not see meets weight 0, which an infinity there turns into NaN: a row whose
 // result is not finite is taken again by itself (cache_plain_row).
-// Fewer row tiles than SMs: the positions are cut into parts whose fp32 sums cache_join_kernel joins in order.
+// Few row tiles: the positions are cut into parts whose fp32 sums cache_join_kernel joins in order.  More of them: the blocks, one an SM, share
+// all tiles of positions evenly, whatever the lengths, and copies and conversions of a row tile begin under the results of the one before.
 // Bound: the tensor core and the instructions about the scores together: 2 048 cycles of products for 256 rows and 128 positions of a 128-wide head,
 // as many for their exponentials, and some 5 instructions a score (codes: 6 to 7) on four schedulers.
 #include <algorithm>
@@ -26,8 +27,23 @@
 namespace prism {
 
 constexpr int CT_ROWS = 256, CT_POS = 128, CT_ST = 2, CT_SC = 4;  // slots of scales
+constexpr uint32_t CT_PAIRS = 1024;                            // row tiles of all entries that are dealt by their work
 constexpr int CT_SOFT = 16;                                     // softmax warps: two threads a row, half of the positions each
+// A row tile costs as many units as it has position tiles, but at least a CT_LEAST-th of the longest: with at most CT_ITEMS row tiles an SM a
+// block has at most CT_ITEMS * CT_LEAST + 2 parts.
+constexpr uint32_t CT_LEAST = 4, CT_ITEMS = 8, CT_SEGMENTS = CT_LEAST * CT_ITEMS + 2;
 constexpr float CT_GROW = 3.0f, CT_UP = 12.0f;  // powers of two: what a score may lie above the maximum in use; of the weights in fp16
+// Part of a row tile that a block does.
+struct CtSegment {
+    CacheEntry x;
+    uint32_t item, kh, r0, here, n_q, n;  // row tile of an entry and head, its head, first row, rows, tiles of 128 rows; position tiles of this part
+    int32_t i_lo, first, main;            // the first of them; CtTiles
+    uint32_t whole;                       // the whole row tile
+    uint32_t units, from, take;           // of the row tile, of this part
+    uint32_t b0, b1, slot, slot0;         // blocks that have parts of the item; places of this block's part and of b0's
+    // barriers go on from part to part: position tiles before this one (T1: with a second tile of rows), parts with such tiles, with rows
+    uint32_t T, T1, S0, S1, Q;
+};
 template <int KIND, int HD>
 struct CtCfg {
     static constexpr int PANELS = HD / 64, PANEL = 128 * 128, TILE = PANELS * PANEL;  // 128 rows of 64 values, in the 128-byte swizzle
@@ -36,9 +52,11 @@ struct CtCfg {
     static constexpr int K_OFF = 2 * TILE, V_OFF = K_OFF + CT_ST * TILE, SC_OFF = V_OFF + CT_ST * TILE, BAR_OFF = SC_OFF + CT_SC * SLOT;
     // barriers: kfull, kempty, vfull, vempty [2 each], sfull, pfull, ofull [2 each], qfull, scales [4]
     static constexpr int STATE_OFF = BAR_OFF + 8 * (4 * CT_ST + 7 + CT_SC);
-    static constexpr int X_OFF = STATE_OFF + 16;                                       // what the two threads of a row tell each other
+    static constexpr int X_OFF = STATE_OFF + 24;                                       // what the two threads of a row tell each other
     static constexpr int R_OFF = X_OFF + 2 * 2 * CT_ROWS * 4;                          // CacheRow of each row
-    static constexpr size_t SMEM = R_OFF + CT_ROWS * sizeof(CacheRow) + 1024;
+    static constexpr int PRE_OFF = R_OFF + CT_ROWS * (int)sizeof(CacheRow);            // position tiles of the row tiles before each
+    static constexpr int SEG_OFF = PRE_OFF + (CT_PAIRS + 4) * 4;                       // what the block does
+    static constexpr size_t SMEM = SEG_OFF + CT_SEGMENTS * sizeof(CtSegment) + 1024;
     // behind the softmax warps three that convert (one of them copies, with 16-bit rows) and one of products: five warps a scheduler, 96 registers
     static constexpr int CONV = 96, ISSUER = CT_SOFT + 3, THREADS = (ISSUER + 1) * 32;
     static constexpr int RP = ROWB / 16, STEP = CONV / RP;                             // 16-byte pieces of a row; rows between a thread's pieces
@@ -47,12 +65,40 @@ struct CtCfg {
 
 struct CtDev {
     CacheAttnDev a;
-    uint32_t splits, tiles, box;  // parts of the positions, row tiles of an entry and head, positions of a copy
+    uint32_t splits, tiles, box;  // parts of the positions (0: the blocks share the work, below), row tiles of an entry and head, positions of a copy
     uint32_t pool_rows;           // rows of the pool: one past the last
-    float *part;                  // of the blocks, where there are several of a row tile (CacheJoinDev)
+    float *part;                  // of the blocks, where there are several of a row tile (CacheJoinDev); shared work: two a block
+    unsigned int *count;          // shared work: [row tile of an entry and head], zero between launches
 };
 
 namespace {
+
+// The 128-position tiles that some row of a row tile sees: `first` of them from position 0 on (a.sinks), then those from `main` on.
+struct CtTiles {
+    uint32_t here;              // rows of the tile
+    int32_t first, main, all;   // `all` of them
+};
+// WARP: called by whole warps, which share the rows of a tree.
+template <bool WARP>
+__device__ __forceinline__ CtTiles ct_tiles(const CacheAttnDev &a, const CacheEntry &x, uint32_t tile) {
+    const uint32_t n_rows = x.n * a.group, r0 = tile * CT_ROWS;
+    CtTiles t{r0 < n_rows ? min((uint32_t)CT_ROWS, n_rows - r0) : 0, 0, 0, 0};
+    if (t.here == 0) return t;
+    const uint32_t tok_lo = r0 / a.group, tok_hi = (r0 + t.here - 1) / a.group;
+    int32_t low = -1;
+    if (a.window && !a.tree) low = cache_row(a, x, tok_lo).low;
+    else if (a.window) {
+        low = x.len;
+        for (uint32_t i = tok_lo + (WARP ? threadIdx.x & 31 : 0); i <= tok_hi; i += WARP ? 32 : 1) low = min(low, cache_row(a, x, i).low);
+        if (WARP) low = __reduce_min_sync(0xFFFFFFFFu, low);
+    }
+    const int32_t end = a.tree ? x.len : min(x.len, x.first + (int32_t)tok_hi + 1), start = a.tree ? min(low + 1, max(x.first, 0)) : low + 1;
+    const int32_t main_hi = end > 0 ? (end + CT_POS - 1) / CT_POS : 0;
+    t.first = end > 0 ? (int32_t)(min((uint32_t)end, a.sinks) + CT_POS - 1) / CT_POS : 0;
+    t.main = max(start / CT_POS, t.first);
+    t.all = t.first + max(main_hi - t.main, 0);
+    return t;
+}
 
 __device__ __forceinline__ float ct_ex2(float x) {
     float y;
@@ -180,6 +226,138 @@ __device__ __forceinline__ void ct_convert(uint32_t tile, uint32_t flip, const u
     }
 }
 
+// The results of a row tile's part that this thread's row has, half of the columns: stored, or left as a part, which the last block to arrive joins.
+// A function of its own: inlined into the loop over parts it took some 350 registers more than there are.
+template <int KIND, int HD>
+__device__ __noinline__ void ct_results(const CtDev &d, const CtSegment &g, uint8_t *sm, uint32_t o_col, uint32_t warp, uint32_t lane, uint32_t mine, float m,
+                                        float l, int32_t ref) {
+    using C = CtCfg<KIND, HD>;
+    constexpr bool CODES = KIND >= KV_INT8;
+    const CacheAttnDev &a = d.a;
+    const uint32_t q = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane, tid = warp * 32 + lane;
+    const bool there = q * 128 + row < g.here;
+    volatile uint32_t *last_flag = reinterpret_cast<volatile uint32_t *>(sm + C::STATE_OFF + 16);
+    float *xch = reinterpret_cast<float *>(sm + C::X_OFF) + q * 128 + row;
+    auto other = [&](float v, uint32_t turn) {
+        xch[(turn * 2 + half) * CT_ROWS] = v;
+        asm volatile("bar.sync %0, 64;\n" ::"r"(1 + q * 4 + (warp & 3)) : "memory");
+        return xch[(turn * 2 + (half ^ 1)) * CT_ROWS];
+    };
+    // ---- results, half of the columns a thread: O times 2^(ref - 13) where V was over a power of two, as the weights' sum is 2^12-fold ----
+    const float unit = CODES ? ct_pow2(ref - 13) : 1.0f;
+    float inv = 1.0f / l, odd = l > 0.0f ? 0.0f : 1.0f;        // not 0 once an output was not finite
+    const uint32_t rr = g.r0 + q * 128 + row;
+    uint16_t *dst = a.out + (size_t)(g.x.row0 + rr / a.group) * a.out_stride + (size_t)(g.kh * a.group + rr % a.group) * HD + half * (HD / 2);  // of rows that are there
+    auto store = [&](int c, const float (&o)[32]) {            // 32 columns
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float u = o[ct_col<KIND>(2 * i)] * inv, v = o[ct_col<KIND>(2 * i + 1)] * inv;
+            odd = fmaf(u, 0.0f, fmaf(v, 0.0f, odd));
+            w[i] = kv_round2(u, v, a.c.rows_bf16);
+        }
+        if (there)
+#pragma unroll
+            for (int i = 0; i < 4; i++) reinterpret_cast<uint4 *>(dst + c * 32)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    };
+    bool done = g.whole;
+    if (g.whole) {
+#pragma unroll 1
+        for (int c = 0; c < HD / 64; c++) {
+            uint32_t o[32];
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] = 0;
+            if (mine) {
+                t5::ld32(o_col + c * 32, o);
+                t5::wait_ld();
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i++) v[i] = __uint_as_float(o[i]) * unit;
+            store(c, v);
+            __syncwarp();                                      // the next TMEM read takes the whole warp
+        }
+    } else {
+        constexpr size_t PART = cache_part_floats(CT_ROWS, HD);
+        const size_t at = q * 128 + row, c_first = half * (HD / 8);  // groups of four columns
+        float *to = d.part + g.slot * PART;
+#pragma unroll 1
+        for (int c = 0; c < HD / 64; c++) {
+            uint32_t o[32];
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] = 0;
+            if (mine) {
+                t5::ld32(o_col + c * 32, o);
+                t5::wait_ld();
+            }
+            if (there) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const auto col = [&](int k) { return __uint_as_float(o[ct_col<KIND>(4 * i + k)]) * unit; };
+                    const float4 v = make_float4(col(0), col(1), col(2), col(3));
+                    __stcg(reinterpret_cast<float4 *>(to) + (c_first + c * 8 + i) * CT_ROWS + at, v);
+                }
+            }
+            __syncwarp();
+        }
+        if (half == 0) {
+            __stcg(to + CT_ROWS * HD + at, m);
+            __stcg(to + CT_ROWS * (HD + 1) + at, l);
+        }
+        if (d.splits == 0) {                                   // else cache_join_kernel follows
+            __threadfence();
+            asm volatile("bar.sync 10, 512;\n" ::: "memory");
+            if (tid == 0) {
+                const bool last = atomicAdd(d.count + g.item, 1u) == g.b1 - g.b0;
+                if (last) d.count[g.item] = 0;                   // for the next launch
+                *last_flag = last;
+            }
+            asm volatile("bar.sync 10, 512;\n" ::: "memory");
+            done = *last_flag;
+            if (done && q < g.n_q) {
+                const uint32_t b0 = g.b0, b1 = g.b1;
+                __threadfence();
+                auto part = [&](uint32_t b) { return d.part + (b == b0 ? g.slot0 : 2 * b) * PART + at; };
+                float best = -INFINITY;
+                for (uint32_t b = b0; b <= b1; b++) best = fmaxf(best, __ldcg(part(b) + CT_ROWS * HD));
+                const float sub = best == -INFINITY ? 0.0f : best;
+                l = 0.0f;
+                for (uint32_t b = b0; b <= b1; b++) l += __ldcg(part(b) + CT_ROWS * (HD + 1)) * ct_ex2(__ldcg(part(b) + CT_ROWS * HD) - sub);
+                inv = 1.0f / l;
+                odd = l > 0.0f ? 0.0f : 1.0f;
+#pragma unroll 1
+                for (int c = 0; c < HD / 64; c++) {
+                    float v[32];                               // in the order that store() takes
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = 0.0f;
+                    for (uint32_t b = b0; b <= b1 && there; b++) {
+                        const float f = ct_ex2(__ldcg(part(b) + CT_ROWS * HD) - sub);
+                        const float4 *p = reinterpret_cast<const float4 *>(part(b) - at) + (c_first + c * 8) * CT_ROWS + at;
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float4 u = __ldcg(p + (size_t)i * CT_ROWS);
+                            v[ct_col<KIND>(4 * i)] = fmaf(u.x, f, v[ct_col<KIND>(4 * i)]);
+                            v[ct_col<KIND>(4 * i + 1)] = fmaf(u.y, f, v[ct_col<KIND>(4 * i + 1)]);
+                            v[ct_col<KIND>(4 * i + 2)] = fmaf(u.z, f, v[ct_col<KIND>(4 * i + 2)]);
+                            v[ct_col<KIND>(4 * i + 3)] = fmaf(u.w, f, v[ct_col<KIND>(4 * i + 3)]);
+                        }
+                    }
+                    store(c, v);
+                }
+            }
+        }
+    }
+    const float theirs = other(odd, (mine & 1) ^ 1);           // every lane takes part; after what the other thread stored
+    if (done) {
+        const bool again = there && (odd != 0.0f || theirs != 0.0f);
+        if (half == 0)
+            for (uint32_t rows = __ballot_sync(0xFFFFFFFFu, again); rows; rows &= rows - 1) {
+                const uint32_t i = rr - lane + (uint32_t)(__ffs(rows) - 1);
+                cache_plain_row<KIND, HD>(a, g.x, i / a.group, g.kh * a.group + i % a.group, lane);
+            }
+    }
+}
+
 }  // namespace
 
 template <int KIND, int HD>
@@ -216,56 +394,150 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);  // S of tile q at column 128 q, O at 256 + HD q
     pdl_wait();                                                    // before any bounded wait: the kernel before this one may still be at work
 
-    const uint32_t item = blockIdx.x / d.splits, split = blockIdx.x - item * d.splits;
-    const uint32_t tile = item % d.tiles, kh = item / d.tiles % a.c.kv_heads, e = item / d.tiles / a.c.kv_heads;
-    CacheEntry x;
-    const bool is = cache_entry(a, e, x);                          // the same in all blocks of an item
-    const uint32_t n_rows = is ? x.n * a.group : 0, r0 = tile * CT_ROWS;
-    const uint32_t here = r0 < n_rows ? min((uint32_t)CT_ROWS, n_rows - r0) : 0, n_q = (here + 127) / 128;
-    // ---- the positions that some row sees: the first tiles (a.sinks), then main_lo .. --------------------------------------
-    int32_t i_lo = 0, i_hi = 0, first_tiles = 0, main_lo = 0;
-    if (here) {
-        const uint32_t tok_lo = r0 / a.group, tok_hi = (r0 + here - 1) / a.group;
-        int32_t low = -1;
-        if (a.window && !a.tree) low = cache_row(a, x, tok_lo).low;
-        else if (a.window) {
-            low = x.len;
-            for (uint32_t i = tok_lo + lane; i <= tok_hi; i += 32) low = min(low, cache_row(a, x, i).low);
-            low = __reduce_min_sync(0xFFFFFFFFu, low);
+    // ---- what this block does ----------------------------------------------------------------------------------------------
+    // d.splits > 0: one part of one row tile.  Else all blocks share the position tiles of all row tiles evenly, in order: a block has the rest of
+    // a row tile, whole ones, the beginning of another.  Row tile i of entry e is pair e * d.tiles + i, an item is a pair and a head.
+    uint32_t *pre = reinterpret_cast<uint32_t *>(smem + C::PRE_OFF);
+    CtSegment *segs = reinterpret_cast<CtSegment *>(smem + C::SEG_OFF);
+    {
+        const uint32_t kvh = a.c.kv_heads, pairs = a.n_entries * d.tiles;
+        if (d.splits == 0) {
+            for (uint32_t i = tid; i < pairs; i += C::THREADS) {
+                CacheEntry x;
+                uint32_t c = 0;
+                if (cache_entry(a, i / d.tiles, x)) {
+                    const CtTiles t = ct_tiles<false>(a, x, i % d.tiles);
+                    if (t.here) c = (uint32_t)max(t.all, 1);       // rows that see nothing are results, too
+                }
+                pre[i + 1] = c;
+            }
+            __syncthreads();
+            if (warp == 0) {
+                const uint32_t per = (pairs + 31) / 32, lo = min(lane * per, pairs), hi = min(lo + per, pairs);
+                uint32_t longest = 0, sum = 0;
+                for (uint32_t i = lo; i < hi; i++) longest = max(longest, pre[i + 1]);
+                longest = __reduce_max_sync(0xFFFFFFFFu, longest);
+                auto cost = [&](uint32_t c) { return c ? max(c, (longest + CT_LEAST - 1) / CT_LEAST) : 0; };
+                for (uint32_t i = lo; i < hi; i++) sum += cost(pre[i + 1]);
+                uint32_t all = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, all, o);
+                    if (lane >= (uint32_t)o) all += v;
+                }
+                sum = all - sum;
+                if (lane == 0) pre[0] = 0;
+                for (uint32_t i = lo; i < hi; i++) pre[i + 1] = sum += cost(pre[i + 1]);
+                __syncwarp();
+                if (lane == 0) {
+                    const uint64_t total = (uint64_t)pre[pairs] * kvh, G = min((uint64_t)gridDim.x, total);  // every block of G has a unit
+                    const uint64_t end = blockIdx.x < G ? total * (blockIdx.x + 1) / G : 0;
+                    uint64_t at = blockIdx.x < G ? total * blockIdx.x / G : 0;
+                    uint32_t k = 0, p = 0, hi2 = pairs;
+                    while (hi2 - p > 1) {                          // the last pair that begins at or before this unit
+                        const uint32_t mid = (p + hi2) / 2;
+                        if ((uint64_t)pre[mid] * kvh <= at) p = mid;
+                        else hi2 = mid;
+                    }
+                    for (; at < end && k < CT_SEGMENTS; k++) {
+                        while ((uint64_t)pre[p + 1] * kvh <= at) p++;
+                        CtSegment &g = segs[k];
+                        const uint32_t units = pre[p + 1] - pre[p], in = (uint32_t)(at - (uint64_t)pre[p] * kvh);
+                        g.kh = in / units;
+                        g.item = p * kvh + g.kh;
+                        g.units = units;
+                        g.from = in % units;
+                        g.take = (uint32_t)min((uint64_t)(units - g.from), end - at);
+                        g.whole = g.take == units;
+                        const uint64_t item_unit = at - g.from;
+                        g.b0 = (uint32_t)(((item_unit + 1) * G - 1) / total);
+                        g.b1 = (uint32_t)(((item_unit + units) * G - 1) / total);
+                        g.slot0 = 2 * g.b0 + (total * g.b0 / G < item_unit);  // a block's first part, or its last
+                        g.slot = blockIdx.x == g.b0 ? g.slot0 : 2 * blockIdx.x;
+                        at += g.take;
+                    }
+                    pre[CT_PAIRS + 1] = k;
+                }
+            }
+        } else if (tid == 0) {
+            CtSegment &g = segs[0];
+            g.item = blockIdx.x / d.splits;
+            g.kh = g.item / d.tiles % kvh;
+            g.whole = d.splits == 1;
+            g.slot = blockIdx.x;
+            g.units = d.splits;
+            g.from = blockIdx.x % d.splits;
+            g.take = 1;
+            pre[CT_PAIRS + 1] = 1;
         }
-        const int32_t end = a.tree ? x.len : min(x.len, x.first + (int32_t)tok_hi + 1), start = a.tree ? min(low + 1, max(x.first, 0)) : low + 1;
-        const int32_t main_hi = end > 0 ? (end + CT_POS - 1) / CT_POS : 0;
-        first_tiles = end > 0 ? (int32_t)(min((uint32_t)end, a.sinks) + CT_POS - 1) / CT_POS : 0;
-        main_lo = max(start / CT_POS, first_tiles);
-        const int32_t n_tiles = first_tiles + max(main_hi - main_lo, 0);
-        i_lo = (int32_t)((int64_t)n_tiles * split / d.splits);
-        i_hi = (int32_t)((int64_t)n_tiles * (split + 1) / d.splits);
+        __syncthreads();
+        for (uint32_t k = warp; k < pre[CT_PAIRS + 1]; k += C::THREADS / 32) {
+            CtSegment &g = segs[k];
+            const uint32_t pair = d.splits ? g.item / d.tiles / kvh * d.tiles + g.item % d.tiles : g.item / kvh;
+            CacheEntry x{};
+            CtTiles t{};
+            if (cache_entry(a, pair / d.tiles, x)) t = ct_tiles<true>(a, x, pair % d.tiles);  // the same in all blocks of an item
+            if (lane == 0) {
+                g.x = x;
+                g.r0 = pair % d.tiles * CT_ROWS;
+                g.here = t.here;
+                g.n_q = (t.here + 127) / 128;
+                g.first = t.first;
+                g.main = t.main;
+                g.i_lo = (int32_t)((int64_t)t.all * g.from / g.units);
+                g.n = (uint32_t)((int32_t)((int64_t)t.all * (g.from + g.take) / g.units) - g.i_lo);
+            }
+        }
+        __syncthreads();
+        if (tid == 0) {
+            uint32_t T = 0, T1 = 0, S0 = 0, S1 = 0, Q = 0;
+            for (uint32_t k = 0; k < pre[CT_PAIRS + 1]; k++) {
+                CtSegment &g = segs[k];
+                g.T = T;
+                g.T1 = T1;
+                g.S0 = S0;
+                g.S1 = S1;
+                g.Q = Q;
+                T += g.n;
+                T1 += g.n_q == 2 ? g.n : 0;
+                S0 += g.n > 0;
+                S1 += g.n > 0 && g.n_q == 2;
+                Q += g.here > 0;
+            }
+            pre[CT_PAIRS + 2] = T;
+        }
+        __syncthreads();
     }
-    const uint32_t n = (uint32_t)(i_hi - i_lo);
-    auto pos_of = [&](uint32_t j) {
-        const int32_t i = i_lo + (int32_t)j;
-        return (i < first_tiles ? i : main_lo + (i - first_tiles)) * CT_POS;
+    const uint32_t n_segs = pre[CT_PAIRS + 1];
+    auto pos_of = [](const CtSegment &g, uint32_t j) {
+        const int32_t i = g.i_lo + (int32_t)j;
+        return (i < g.first ? i : g.main + (i - g.first)) * CT_POS;
     };
 
-    if (here == 0) {
-        // nothing of this entry
-    } else if (warp < CT_SOFT) {
+    if (warp < CT_SOFT) {
         // ================= softmax: two threads a query row, positions 0..63 and 64..127 of a tile =================
-        const uint32_t q = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane, lanes = ((warp & 3) * 32) << 16, rr = r0 + q * 128 + row;
-        const uint32_t s_col = tmem + lanes + q * 128, o_col = tmem + lanes + 256 + q * HD + half * (HD / 2);
-        const bool there = q * 128 + row < here;
-        float *xch = reinterpret_cast<float *>(smem + C::X_OFF) + q * 128 + row;  // [turn][half][256 rows]
+        for (uint32_t k = 0; k < n_segs; k++) {
+        // Taken anew for every part: kept over the loop, what follows from them would take more registers than there are.
+        uint32_t w_now = warp, l_now = lane, t_now = tmem, s_now = 0;
+        asm volatile("" : "+r"(w_now), "+r"(l_now), "+r"(t_now), "+r"(s_now));
+        uint8_t *const sm = smem + s_now;
+        const uint32_t q = w_now >> 3, half = w_now >> 2 & 1, row = (w_now & 3) * 32 + l_now, lanes = ((w_now & 3) * 32) << 16;
+        const uint32_t s_col = t_now + lanes + q * 128, o_col = t_now + lanes + 256 + q * HD + half * (HD / 2);
+        float *xch = reinterpret_cast<float *>(sm + C::X_OFF) + q * 128 + row;  // [turn][half][256 rows]
         // The value of the row's other thread.  Turns alternate: both have read one turn's before either writes it again.
         auto other = [&](float v, uint32_t turn) {
             xch[(turn * 2 + half) * CT_ROWS] = v;
-            asm volatile("bar.sync %0, 64;\n" ::"r"(1 + q * 4 + (warp & 3)) : "memory");
+            asm volatile("bar.sync %0, 64;\n" ::"r"(1 + q * 4 + (w_now & 3)) : "memory");
             return xch[(turn * 2 + (half ^ 1)) * CT_ROWS];
         };
-        CacheRow *row_at = reinterpret_cast<CacheRow *>(smem + C::R_OFF) + q * 128 + row;  // the same in both threads
+        CacheRow *row_at = reinterpret_cast<CacheRow *>(sm + C::R_OFF) + q * 128 + row;  // the same in both threads
+        const CtSegment &g = *(reinterpret_cast<const CtSegment *>(sm + C::SEG_OFF) + k);
+        if (g.here == 0) continue;
+        const bool there = q * 128 + row < g.here;
         int32_t all_to, all_low;
         {
             CacheRow r{0x7FFFFFF0, -1, nullptr};                   // a row that is not there: sees everything, is not stored
-            if (there) r = cache_row(a, x, rr / a.group);
+            if (there) r = cache_row(a, g.x, (g.r0 + q * 128 + row) / a.group);
             all_to = __reduce_min_sync(0xFFFFFFFFu, r.last);
             all_low = __reduce_max_sync(0xFFFFFFFFu, r.low);
             *row_at = r;
@@ -273,9 +545,9 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         float mul = fabsf(a.scale) * 1.4426950408889634f, qsum = 0.0f;
         {   // half of the row of q into its tile, its sign that of the scale
             constexpr int W = HD / 16;
-            const uint32_t token = there ? rr / a.group : 0, head = kh * a.group + (there ? rr % a.group : 0);
+            const uint32_t rr = g.r0 + q * 128 + row, token = there ? rr / a.group : 0, head = g.kh * a.group + (there ? rr % a.group : 0);
             const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-            const uint4 *src = reinterpret_cast<const uint4 *>(a.q + (size_t)(x.row0 + token) * a.q_stride + (size_t)head * HD) + half * W;
+            const uint4 *src = reinterpret_cast<const uint4 *>(a.q + (size_t)(g.x.row0 + token) * a.q_stride + (size_t)head * HD) + half * W;
             uint4 w[W];
             float big = 0.0f;
 #pragma unroll
@@ -310,31 +582,31 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
 #pragma unroll
             for (int i = 0; i < W; i++) {
                 const uint32_t c = half * W + i;
-                *reinterpret_cast<uint4 *>(smem + q * C::TILE + (c >> 3) * C::PANEL + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = ct_order<KIND>(w[i]);
+                *reinterpret_cast<uint4 *>(sm + q * C::TILE + (c >> 3) * C::PANEL + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = ct_order<KIND>(w[i]);
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            asm volatile("bar.sync %0, 64;\n" ::"r"(1 + q * 4 + (warp & 3)) : "memory");  // the exchanged values have been read
-            if (lane == 0) t5::mbar_arrive(b_qfull);
+            asm volatile("bar.sync %0, 64;\n" ::"r"(1 + q * 4 + (w_now & 3)) : "memory");  // the exchanged values have been read
+            if (l_now == 0) t5::mbar_arrive(b_qfull);
         }
         float m = -INFINITY, l = 0.0f;
         int32_t ref = 0;                                           // exponent that O is over
-        const uint32_t mine = q < n_q ? n : 0;
+        const uint32_t mine = q < g.n_q ? g.n : 0, T = g.T, Tq = q ? g.T1 : T;
         for (uint32_t j = 0; j < mine; j++) {
             int32_t ex = 0;
             const float *ksc = nullptr;
             if constexpr (CODES) {
-                t5::mbar_wait_warp(b_sc + 8 * (j % CT_SC), (j / CT_SC) & 1, err_flag);
-                ksc = reinterpret_cast<const float *>(smem + C::SC_OFF + (j % CT_SC) * C::SLOT);
+                t5::mbar_wait_warp(b_sc + 8 * ((T + j) % CT_SC), ((T + j) / CT_SC) & 1, err_flag);
+                ksc = reinterpret_cast<const float *>(sm + C::SC_OFF + ((T + j) % CT_SC) * C::SLOT);
                 ex = ct_exponent(ksc + 2 * CT_POS * NSC);
                 ksc += half * 64 * NSC;
             }
-            t5::mbar_wait_warp(b_sfull + 8 * q, j & 1, err_flag);
+            t5::mbar_wait_warp(b_sfull + 8 * q, (Tq + j) & 1, err_flag);
             t5::fence_after();
             uint32_t s[2][32];
 #pragma unroll
             for (int c = 0; c < 2; c++) t5::ld32(s_col + half * 64 + c * 32, s[c]);
             t5::wait_ld();
-            const int32_t p0 = pos_of(j) + (int32_t)half * 64;
+            const int32_t p0 = pos_of(g, j) + (int32_t)half * 64;
             if constexpr (NSC == 1) {
 #pragma unroll
                 for (int c = 0; c < 2; c++)
@@ -359,7 +631,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             if (p0 + 63 > all_to || !(p0 > all_low || (uint32_t)(p0 + 64) <= a.sinks)) {  // some row of the warp does not see all 64
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    const uint32_t see = there ? ct_seen(a, x, *row_at, p0 + c * 32) : 0xFFFFFFFFu;
+                    const uint32_t see = there ? ct_seen(a, g.x, *row_at, p0 + c * 32) : 0xFFFFFFFFu;
 #pragma unroll
                     for (int i = 0; i < 32; i++)
                         if (!(see & (1u << i))) s[c][i] = 0xFF800000u;
@@ -425,85 +697,25 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             t5::wait_st();
             t5::fence_before();
             __syncwarp();
-            if (lane == 0) t5::mbar_arrive(b_pfull + 8 * q);
+            if (l_now == 0) t5::mbar_arrive(b_pfull + 8 * q);
         }
         l += other(l, mine & 1);
         if (mine) {
-            t5::mbar_wait_warp(b_ofull + 8 * q, 0, err_flag);
+            t5::mbar_wait_warp(b_ofull + 8 * q, (q ? g.S1 : g.S0) & 1, err_flag);
             t5::fence_after();
         }
-        // ---- results, half of the columns a thread: O times 2^(ref - 13) where V was over a power of two, as the weights' sum is 2^12-fold ----
-        const float unit = CODES ? ct_pow2(ref - 13) : 1.0f;
-        float inv = 1.0f / l, odd = l > 0.0f ? 0.0f : 1.0f;        // not 0 once an output was not finite
-        uint16_t *dst = there ? a.out + (size_t)(x.row0 + rr / a.group) * a.out_stride + (size_t)(kh * a.group + rr % a.group) * HD + half * (HD / 2) : nullptr;
-        auto store = [&](int c, const float (&o)[32]) {            // 32 columns
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float u = o[ct_col<KIND>(2 * i)] * inv, v = o[ct_col<KIND>(2 * i + 1)] * inv;
-                odd = fmaf(u, 0.0f, fmaf(v, 0.0f, odd));
-                w[i] = kv_round2(u, v, a.c.rows_bf16);
-            }
-            if (there)
-#pragma unroll
-                for (int i = 0; i < 4; i++) reinterpret_cast<uint4 *>(dst + c * 32)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-        };
-        if (d.splits == 1) {
-#pragma unroll 1
-            for (int c = 0; c < HD / 64; c++) {
-                uint32_t o[32];
-                float v[32];
-                if (mine) {
-                    t5::ld32(o_col + c * 32, o);
-                    t5::wait_ld();
-                }
-#pragma unroll
-                for (int i = 0; i < 32; i++) v[i] = mine ? __uint_as_float(o[i]) * unit : 0.0f;
-                store(c, v);
-                __syncwarp();                                      // the next TMEM read takes the whole warp
-            }
-        } else {
-            const size_t at = q * 128 + row, c_first = half * (HD / 8);  // groups of four columns
-            float *to = d.part + (size_t)blockIdx.x * cache_part_floats(CT_ROWS, HD);
-#pragma unroll 1
-            for (int c = 0; c < HD / 64; c++) {
-                uint32_t o[32];
-                if (mine) {
-                    t5::ld32(o_col + c * 32, o);
-                    t5::wait_ld();
-                }
-                if (there) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const auto col = [&](int k) { return mine ? __uint_as_float(o[ct_col<KIND>(4 * i + k)]) * unit : 0.0f; };
-                        const float4 v = make_float4(col(0), col(1), col(2), col(3));
-                        __stcg(reinterpret_cast<float4 *>(to) + (c_first + c * 8 + i) * CT_ROWS + at, v);
-                    }
-                }
-                __syncwarp();
-            }
-            if (half == 0) {
-                __stcg(to + CT_ROWS * HD + at, m);
-                __stcg(to + CT_ROWS * (HD + 1) + at, l);
-            }
-        }
-        if (d.splits == 1) {
-            const float theirs = other(odd, (mine & 1) ^ 1);       // every lane takes part; after what the other thread stored
-            const bool again = there && (odd != 0.0f || theirs != 0.0f);
-            if (half == 0)
-                for (uint32_t rows = __ballot_sync(0xFFFFFFFFu, again); rows; rows &= rows - 1) {
-                    const uint32_t i = rr - lane + (uint32_t)(__ffs(rows) - 1);
-                    cache_plain_row<KIND, HD>(a, x, i / a.group, kh * a.group + i % a.group, lane);
-                }
-        }
+        ct_results<KIND, HD>(d, g, sm, o_col, w_now, l_now, mine, m, l, ref);
         t5::fence_before();
+        // the next segment's first exchange takes a turn whose last readers have been at this barrier
+        asm volatile("bar.sync %0, 64;\n" ::"r"(1 + q * 4 + (w_now & 3)) : "memory");
+        }
     } else if (warp == C::ISSUER) {
         // ================= products: the whole warp walks the tiles (descriptors stay in uniform registers), an elected lane issues;
         // all lanes clear 16-bit value rows past the end =================
         const uint32_t types = BF16 ? 1u << 7 | 1u << 10 : 0u;
         const uint32_t id_s = t5::idesc_f16(128, CT_POS) | types, id_o = t5::idesc_f16(128, HD) | types | (1u << 16);  // V is read across its rows
-        auto scores = [&](uint32_t q, uint32_t j) {
-            const uint32_t qa = base + q * C::TILE, ka = base + C::K_OFF + (j % ST) * C::TILE;
+        auto scores = [&](uint32_t q, uint32_t J) {                // J: of all segments
+            const uint32_t qa = base + q * C::TILE, ka = base + C::K_OFF + (J % ST) * C::TILE;
 #pragma unroll
             for (int k = 0; k < HD / 16; k++) {
                 const uint32_t off = (k * 32 / 128) * C::PANEL + (k * 32) % 128;
@@ -511,54 +723,59 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             }
             t5::commit(b_sfull + 8 * q);
         };
-        if (n) {
-            t5::mbar_wait_bounded(b_qfull, 0, err_flag);
-            t5::mbar_wait_bounded(b_kfull, 0, err_flag);
-            __syncwarp();
-            t5::fence_after();
-            if (t5::elect_one()) {
-                for (uint32_t q = 0; q < n_q; q++) scores(q, 0);
-                t5::commit(b_kempty);
-            }
-            __syncwarp();
-        }
-        for (uint32_t j = 0; j < n; j++) {
-            const uint32_t st = j % ST, ph = (j / ST) & 1, va = base + C::V_OFF + st * C::TILE, jn = j + 1;
-            t5::mbar_wait_bounded(b_vfull + 8 * st, ph, err_flag);
-            __syncwarp();
-            if constexpr (!CODES) {
-                const int32_t left = x.len - pos_of(j);
-                if (left < CT_POS) {
-                    const uint32_t first = (uint32_t)left, cells = (CT_POS - first) * 8 * C::PANELS;
-                    for (uint32_t i = lane; i < cells; i += 32) {
-                        const uint32_t p = i / ((CT_POS - first) * 8), c = i % ((CT_POS - first) * 8);
-                        *reinterpret_cast<uint4 *>(smem + C::V_OFF + st * C::TILE + p * C::PANEL + first * 128 + c * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                    __syncwarp();
-                }
-            }
-            if (jn < n) t5::mbar_wait_bounded(b_kfull + 8 * (jn % ST), (jn / ST) & 1, err_flag);
-#pragma unroll
-            for (uint32_t q = 0; q < 2; q++) {
-                if (q >= n_q) continue;
-                t5::mbar_wait_bounded(b_pfull + 8 * q, j & 1, err_flag);
+        for (uint32_t i = 0; i < n_segs; i++) {
+            const CtSegment &g = segs[i];
+            const uint32_t n = g.n, n_q = g.n_q, T = g.T, T1 = g.T1;
+            if (n) {
+                t5::mbar_wait_bounded(b_qfull, g.Q & 1, err_flag);
+                t5::mbar_wait_bounded(b_kfull + 8 * (T % ST), (T / ST) & 1, err_flag);
                 __syncwarp();
                 t5::fence_after();
                 if (t5::elect_one()) {
-#pragma unroll
-                    for (int k = 0; k < CT_POS / 16; k++)
-                        t5::mma_ts(tmem + 256 + q * HD, tmem + q * 128 + k * 8, t5::desc_swizzled<128>(va + k * 16 * 128, C::PANEL), id_o, k ? 1u : j);
-                    if (jn < n) scores(q, jn);
-                    else t5::commit(b_ofull + 8 * q);
+                    for (uint32_t q = 0; q < n_q; q++) scores(q, T);
+                    t5::commit(b_kempty + 8 * (T % ST));
                 }
                 __syncwarp();
             }
-            if (t5::elect_one()) {
-                t5::commit(b_vempty + 8 * st);
-                if (jn < n) t5::commit(b_kempty + 8 * (jn % ST));
+            for (uint32_t j = 0; j < n; j++) {
+                const uint32_t J = T + j, st = J % ST, ph = (J / ST) & 1, va = base + C::V_OFF + st * C::TILE;
+                const bool more = j + 1 < n;
+                t5::mbar_wait_bounded(b_vfull + 8 * st, ph, err_flag);
+                __syncwarp();
+                if constexpr (!CODES) {
+                    const int32_t left = g.x.len - pos_of(g, j);
+                    if (left < CT_POS) {
+                        const uint32_t first = (uint32_t)left, cells = (CT_POS - first) * 8 * C::PANELS;
+                        for (uint32_t u = lane; u < cells; u += 32) {
+                            const uint32_t p = u / ((CT_POS - first) * 8), c = u % ((CT_POS - first) * 8);
+                            *reinterpret_cast<uint4 *>(smem + C::V_OFF + st * C::TILE + p * C::PANEL + first * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                        __syncwarp();
+                    }
+                }
+                if (more) t5::mbar_wait_bounded(b_kfull + 8 * ((J + 1) % ST), ((J + 1) / ST) & 1, err_flag);
+#pragma unroll
+                for (uint32_t q = 0; q < 2; q++) {
+                    if (q >= n_q) continue;
+                    t5::mbar_wait_bounded(b_pfull + 8 * q, ((q ? T1 : T) + j) & 1, err_flag);
+                    __syncwarp();
+                    t5::fence_after();
+                    if (t5::elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < CT_POS / 16; k++)
+                            t5::mma_ts(tmem + 256 + q * HD, tmem + q * 128 + k * 8, t5::desc_swizzled<128>(va + k * 16 * 128, C::PANEL), id_o, k ? 1u : j);
+                        if (more) scores(q, J + 1);
+                        else t5::commit(b_ofull + 8 * q);
+                    }
+                    __syncwarp();
+                }
+                if (t5::elect_one()) {
+                    t5::commit(b_vempty + 8 * st);
+                    if (more) t5::commit(b_kempty + 8 * ((J + 1) % ST));
+                }
+                __syncwarp();
             }
-            __syncwarp();
         }
         t5::fence_before();
     } else if constexpr (!CODES) {
@@ -566,9 +783,9 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         // A lane a box (of at most eight): its page is asked for a tile before it is needed.
         if (warp == CT_SOFT) {
             const uint32_t boxes = CT_POS / d.box, b = lane % boxes;
-            auto look = [&](uint32_t j) {
-                const int32_t p = j < n ? pos_of(j) + (int32_t)(b * d.box) : x.len;
-                return p < x.len ? kv_page_number(a.c, x.seq, (uint32_t)p) : 0xFFFFFFFFu;
+            auto look = [&](const CtSegment &g, uint32_t j) {
+                const int32_t p = j < g.n ? pos_of(g, j) + (int32_t)(b * d.box) : g.x.len;
+                return p < g.x.len ? kv_page_number(a.c, g.x.seq, (uint32_t)p) : 0xFFFFFFFFu;
             };
             auto load = [&](const CUtensorMap *map, uint32_t dst, uint32_t at, uint32_t mbar) {
                 if (lane == 0) t5::mbar_arrive_expect_tx(mbar, CT_POS * HD * 2);
@@ -577,20 +794,24 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                     for (uint32_t q = 0; q < (uint32_t)C::PANELS; q++)
                         t5::tma_2d(dst + q * C::PANEL + b * d.box * 128, map, (int32_t)(q * 64), (int32_t)at, mbar);
             };
-            uint32_t page = look(0);
-            for (uint32_t j = 0; j < n; j++) {
-                const uint32_t st = j % ST, ph = (j / ST) & 1;
-                const int32_t p = pos_of(j) + (int32_t)(b * d.box);
-                // past the last row of the pool: zeros
-                const uint32_t at = p < x.len && kv_page_ok(a.c, page) ? (uint32_t)kv_row(a.c, page, kh, (uint32_t)p) : d.pool_rows;
-                page = look(j + 1);
-                t5::mbar_wait_warp(b_kempty + 8 * st, ph ^ 1, err_flag);
-                load(&kmap, base + C::K_OFF + st * C::TILE, at, b_kfull + 8 * st);
-                t5::mbar_wait_warp(b_vempty + 8 * st, ph ^ 1, err_flag);
-                load(&vmap, base + C::V_OFF + st * C::TILE, at, b_vfull + 8 * st);
+            for (uint32_t k = 0; k < n_segs; k++) {
+                const CtSegment &g = segs[k];
+                uint32_t page = look(g, 0);
+                for (uint32_t j = 0; j < g.n; j++) {
+                    const uint32_t st = (g.T + j) % ST, ph = ((g.T + j) / ST) & 1;
+                    const int32_t p = pos_of(g, j) + (int32_t)(b * d.box);
+                    // past the last row of the pool: zeros
+                    const uint32_t at = p < g.x.len && kv_page_ok(a.c, page) ? (uint32_t)kv_row(a.c, page, g.kh, (uint32_t)p) : d.pool_rows;
+                    page = look(g, j + 1);
+                    t5::mbar_wait_warp(b_kempty + 8 * st, ph ^ 1, err_flag);
+                    load(&kmap, base + C::K_OFF + st * C::TILE, at, b_kfull + 8 * st);
+                    t5::mbar_wait_warp(b_vempty + 8 * st, ph ^ 1, err_flag);
+                    load(&vmap, base + C::V_OFF + st * C::TILE, at, b_vfull + 8 * st);
+                }
             }
             // every copy in flight lands before the CTA leaves
-            for (uint32_t j = n > (uint32_t)ST ? n - ST : 0; j < n; j++) {
+            const uint32_t T = pre[CT_PAIRS + 2];
+            for (uint32_t j = T > (uint32_t)ST ? T - ST : 0; j < T; j++) {
                 t5::mbar_wait_warp(b_kfull + 8 * (j % ST), (j / ST) & 1, err_flag);
                 t5::mbar_wait_warp(b_vfull + 8 * (j % ST), (j / ST) & 1, err_flag);
             }
@@ -615,15 +836,15 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         float2 scr[2][2];                                          // keys', values' scales of positions ct and ct + 96
         uint32_t at_k = 0, at_v = 0;                               // lanes 0..7: the pool row of the tile's 16-position unit (0 where there is none)
         // Pages are asked for two tiles ahead, so that nothing waits for the table.
-        auto look = [&](uint32_t j) {
-            const int32_t p = j < n ? pos_of(j) + (int32_t)(lane & 7) * 16 : x.len;
-            return p < x.len ? kv_page_number(a.c, x.seq, (uint32_t)p) : 0xFFFFFFFFu;
+        auto look = [&](const CtSegment &g, uint32_t j) {
+            const int32_t p = j < g.n ? pos_of(g, j) + (int32_t)(lane & 7) * 16 : g.x.len;
+            return p < g.x.len ? kv_page_number(a.c, g.x.seq, (uint32_t)p) : 0xFFFFFFFFu;
         };
-        auto units = [&](uint32_t j, uint32_t page) {
-            const int32_t p = j < n ? pos_of(j) + (int32_t)(lane & 7) * 16 : x.len;
-            return p < x.len && kv_page_ok(a.c, page) ? (uint32_t)kv_row(a.c, page, kh, (uint32_t)p) : 0u;
+        auto units = [&](const CtSegment &g, uint32_t j, uint32_t page) {
+            const int32_t p = j < g.n ? pos_of(g, j) + (int32_t)(lane & 7) * 16 : g.x.len;
+            return p < g.x.len && kv_page_ok(a.c, page) ? (uint32_t)kv_row(a.c, page, g.kh, (uint32_t)p) : 0u;
         };
-        uint32_t page = look(0);
+        uint32_t page;
         // Four pieces at a time, so that what they wait for overlaps.
         constexpr int G = 4;
         auto load = [&](const uint8_t *pool, int first, uint32_t of) {
@@ -635,20 +856,20 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                 if (first + i < MINE) reg[first + i] = t5::ldg128_nc(pool + (size_t)(at[i] + ((row0 + (first + i) * STEP) & 15)) * C::ROWB + piece * 16);
         };
         // Past the end some row of the pool is read; its scale is 0, but a code of e4m3 may be NaN.
-        auto clear = [&](int32_t p0) {
-            if (KIND == KV_E4M3 && p0 + CT_POS > x.len) {
+        auto clear = [&](int32_t p0, int32_t len) {
+            if (KIND == KV_E4M3 && p0 + CT_POS > len) {
 #pragma unroll
                 for (int i = 0; i < MINE; i++)
-                    if (p0 + (int32_t)(row0 + i * STEP) >= x.len) reg[i] = make_uint4(0, 0, 0, 0);
+                    if (p0 + (int32_t)(row0 + i * STEP) >= len) reg[i] = make_uint4(0, 0, 0, 0);
             }
         };
         constexpr int FULL = CT_POS / STEP;                        // pieces that every thread has
-        auto load_scales = [&](int32_t p0, uint32_t of) {
+        auto load_scales = [&](int32_t p0, int32_t len, uint32_t of) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const uint32_t row = ct + h * 96, at = __shfl_sync(0xFFFFFFFFu, of, (row >> 4) & 7);
                 scr[0][h] = scr[1][h] = make_float2(0.0f, 0.0f);
-                if (row < CT_POS && p0 + (int32_t)row < x.len) {
+                if (row < CT_POS && p0 + (int32_t)row < len) {
                     const size_t from = ((size_t)at + (row & 15)) * NSC;
                     if constexpr (NSC == 2) {
                         scr[0][h] = __ldg(reinterpret_cast<const float2 *>(a.c.ks + from));
@@ -660,20 +881,25 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                 }
             }
         };
+        for (uint32_t k = 0; k < n_segs; k++) {
+        const CtSegment &g = segs[k];
+        const uint32_t n = g.n, T = g.T;
+        const int32_t len = g.x.len;
         if (n) {
-            at_k = units(0, page);
-            page = look(1);
+            page = look(g, 0);
+            at_k = units(g, 0, page);
+            page = look(g, 1);
 #pragma unroll
             for (int i = 0; i < MINE; i += G) load(a.c.k, i, at_k);
-            load_scales(pos_of(0), at_k);
+            load_scales(pos_of(g, 0), len, at_k);
         }
         for (uint32_t j = 0; j < n; j++) {
-            const uint32_t st = j % ST, ph = (j / ST) & 1;
-            const int32_t now = pos_of(j), next = j + 1 < n ? pos_of(j + 1) : x.len;  // nothing is loaded from the end on
+            const uint32_t st = (T + j) % ST, ph = ((T + j) / ST) & 1;
+            const int32_t now = pos_of(g, j), next = j + 1 < n ? pos_of(g, j + 1) : len;  // nothing is loaded from the end on
             at_v = at_k;
             t5::mbar_wait_warp(b_kempty + 8 * st, ph ^ 1, err_flag);
             // the slot's last readers, the softmax of tile j - 4, came before the products that have just been waited for
-            float *ksc = reinterpret_cast<float *>(smem + C::SC_OFF + (j % CT_SC) * C::SLOT), *vsc = ksc + CT_POS * NSC, *tops = vsc + CT_POS * NSC;
+            float *ksc = reinterpret_cast<float *>(smem + C::SC_OFF + ((T + j) % CT_SC) * C::SLOT), *vsc = ksc + CT_POS * NSC, *tops = vsc + CT_POS * NSC;
             float big = 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -690,7 +916,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
             if (lane == 0) tops[cw] = big;
             if (ct == 0) tops[3] = 0.0f;                           // ct_exponent reads four
-            t5::mbar_arrive(b_sc + 8 * (j % CT_SC));
+            t5::mbar_arrive(b_sc + 8 * ((T + j) % CT_SC));
             asm volatile("bar.sync 9, 96;\n" ::: "memory");        // the largest of all three warps
             const float unit = ct_pow2(13 - ct_exponent(tops));
 #pragma unroll
@@ -702,42 +928,43 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                     else vsc[row] = sc.x;
                 }
             }
-            at_k = units(j + 1, page);
-            page = look(j + 2);
-            load_scales(next, at_k);
+            at_k = units(g, j + 1, page);
+            page = look(g, j + 2);
+            load_scales(next, len, at_k);
             const uint32_t kt = base + C::K_OFF + st * C::TILE, vt = base + C::V_OFF + st * C::TILE;
-            clear(now);
+            clear(now, len);
 #pragma unroll
-            for (int g = 0; g < MINE; g += G) {
+            for (int f = 0; f < MINE; f += G) {
 #pragma unroll
-                for (int i = g; i < g + G && i < MINE; i++)
+                for (int i = f; i < f + G && i < MINE; i++)
                     if (i < FULL || row0 + i * STEP < CT_POS) ct_convert<KIND, false>(kt + i * STEP * 128, STEP % 8 ? (i & 1) << 6 : 0, to, swap, reg[i], make_float2(1.0f, 0.0f));
-                load(a.c.v, g, at_v);
+                load(a.c.v, f, at_v);
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             t5::mbar_arrive(b_kfull + 8 * st);
             asm volatile("bar.sync 9, 96;\n" ::: "memory");        // the scales of all three warps
             t5::mbar_wait_warp(b_vempty + 8 * st, ph ^ 1, err_flag);
-            const uint32_t v_at = base + C::SC_OFF + (j % CT_SC) * C::SLOT + (CT_POS + row0) * NSC * 4;
-            clear(now);
+            const uint32_t v_at = base + C::SC_OFF + ((T + j) % CT_SC) * C::SLOT + (CT_POS + row0) * NSC * 4;
+            clear(now, len);
 #pragma unroll
-            for (int g = 0; g < MINE; g += G) {
+            for (int f = 0; f < MINE; f += G) {
                 float2 sc[G];
 #pragma unroll
                 for (int i = 0; i < G; i++) {
                     sc[i] = make_float2(0.0f, 0.0f);
-                    if (g + i < MINE && (g + i < FULL || row0 + (g + i) * STEP < CT_POS)) {
-                        if constexpr (NSC == 2) sc[i] = ct_lds2(v_at + (g + i) * STEP * NSC * 4);
-                        else sc[i].x = ct_lds(v_at + (g + i) * STEP * NSC * 4);
+                    if (f + i < MINE && (f + i < FULL || row0 + (f + i) * STEP < CT_POS)) {
+                        if constexpr (NSC == 2) sc[i] = ct_lds2(v_at + (f + i) * STEP * NSC * 4);
+                        else sc[i].x = ct_lds(v_at + (f + i) * STEP * NSC * 4);
                     }
                 }
 #pragma unroll
-                for (int i = g; i < g + G && i < MINE; i++)
-                    if (i < FULL || row0 + i * STEP < CT_POS) ct_convert<KIND, true>(vt + i * STEP * 128, STEP % 8 ? (i & 1) << 6 : 0, to, swap, reg[i], sc[i - g]);
-                load(a.c.k, g, at_k);
+                for (int i = f; i < f + G && i < MINE; i++)
+                    if (i < FULL || row0 + i * STEP < CT_POS) ct_convert<KIND, true>(vt + i * STEP * 128, STEP % 8 ? (i & 1) << 6 : 0, to, swap, reg[i], sc[i - f]);
+                load(a.c.k, f, at_k);
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             t5::mbar_arrive(b_vfull + 8 * st);
+        }
         }
     }
     __syncthreads();
@@ -758,12 +985,16 @@ static int launch_tiles(prism_cuda_ctx *ctx, const CacheAttnDev &a, uint32_t max
     CtDev d{};
     d.a = a;
     d.tiles = (uint32_t)(((uint64_t)a.max_tokens * a.group + CT_ROWS - 1) / CT_ROWS);
-    const uint64_t items = (uint64_t)a.n_entries * a.c.kv_heads * d.tiles;
+    // Few row tiles: each cut into the same number of parts.  From half as many as SMs on: the blocks share the work, whatever the lengths
+    // (a row tile has two or three parts then, and the last block joins them).  More than a block can list: a block a row tile.
+    const uint64_t pairs = (uint64_t)a.n_entries * d.tiles, items = pairs * a.c.kv_heads;
     uint64_t seen = max_length;
     if (a.window) seen = std::min<uint64_t>(seen, (uint64_t)a.window + a.sinks + 2 * CT_POS + CT_ROWS / a.group);
     const uint64_t most = std::max<uint64_t>(1, (seen + CT_POS - 1) / CT_POS);
-    d.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, ctx->sm_count / items));
-    if (items * d.splits > 0x7FFFFFFFull) return fail(ctx, PRISM_E_ARG, "cache_attention: too many rows");
+    const bool share = items * 2 > (uint64_t)ctx->sm_count && pairs <= CT_PAIRS && items <= (uint64_t)ctx->sm_count * CT_ITEMS;
+    d.splits = share ? 0 : (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, ctx->sm_count / items));
+    const uint64_t blocks = share ? (uint64_t)ctx->sm_count : items * d.splits;
+    if (blocks > 0x7FFFFFFFull) return fail(ctx, PRISM_E_ARG, "cache_attention: too many rows");
     const uint64_t rows = ((uint64_t)a.c.n_pages * a.c.kv_heads) << a.c.shift;
     d.box = std::min<uint32_t>(CT_POS, 1u << a.c.shift);
     d.pool_rows = (uint32_t)rows;
@@ -772,8 +1003,9 @@ static int launch_tiles(prism_cuda_ctx *ctx, const CacheAttnDev &a, uint32_t max
         PRISM_TRY(encode_tensor_map(ctx, &k, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.c.k, HD, rows, HD, 64, d.box, CU_TENSOR_MAP_SWIZZLE_128B));
         PRISM_TRY(encode_tensor_map(ctx, &v, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.c.v, HD, rows, HD, 64, d.box, CU_TENSOR_MAP_SWIZZLE_128B));
     }
-    if (d.splits > 1) PRISM_TRY(cache_scratch(ctx, (size_t)(items * d.splits) * cache_part_floats(CT_ROWS, HD) * 4, 0, &d.part, nullptr));
-    launch_pdl(ctx, "cache_tiles_kernel", cache_tiles_kernel<KIND, HD>, dim3((uint32_t)(items * d.splits)), dim3(C::THREADS), C::SMEM, d, k, v);
+    if (d.splits != 1)
+        PRISM_TRY(cache_scratch(ctx, (size_t)(share ? 2 * blocks : blocks) * cache_part_floats(CT_ROWS, HD) * 4, share ? (size_t)items : 0, &d.part, &d.count));
+    launch_pdl(ctx, "cache_tiles_kernel", cache_tiles_kernel<KIND, HD>, dim3((uint32_t)blocks), dim3(C::THREADS), C::SMEM, d, k, v);
     PRISM_TRY(after_launch(ctx, "cache_tiles_kernel"));
     return d.splits > 1 ? launch_cache_join<KIND, HD>(ctx, CacheJoinDev{a, d.splits, d.tiles, CT_ROWS, d.part}) : PRISM_OK;
 }
