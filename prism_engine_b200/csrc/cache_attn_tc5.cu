@@ -105,6 +105,35 @@ __device__ __forceinline__ float ct_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
+// Two fp32 numbers in neighbouring registers, and operations on both at once; the largest of three.
+__device__ __forceinline__ uint64_t ct_two(uint32_t a, uint32_t b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t ct_two(float a, float b) { return ct_two(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ uint32_t ct_first(uint64_t v) { return (uint32_t)v; }
+__device__ __forceinline__ uint32_t ct_second(uint64_t v) { return (uint32_t)(v >> 32); }
+__device__ __forceinline__ uint64_t ct_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t ct_mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t ct_add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float ct_max3(float a, uint32_t b, uint32_t c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+    return d;
+}
 __device__ __forceinline__ uint32_t ct_below(int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 __device__ __forceinline__ float ct_pow2(int32_t e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
 
@@ -598,7 +627,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                 t5::mbar_wait_warp(b_sc + 8 * ((T + j) % CT_SC), ((T + j) / CT_SC) & 1, err_flag);
                 ksc = reinterpret_cast<const float *>(sm + C::SC_OFF + ((T + j) % CT_SC) * C::SLOT);
                 ex = ct_exponent(ksc + 2 * CT_POS * NSC);
-                ksc += half * 64 * NSC;
+                ksc += half * 64;                                  // scales of all positions, then zeros
             }
             t5::mbar_wait_warp(b_sfull + 8 * q, (Tq + j) & 1, err_flag);
             t5::fence_after();
@@ -607,25 +636,26 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             for (int c = 0; c < 2; c++) t5::ld32(s_col + half * 64 + c * 32, s[c]);
             t5::wait_ld();
             const int32_t p0 = pos_of(g, j) + (int32_t)half * 64;
-            if constexpr (NSC == 1) {
+            if constexpr (NSC > 0) {
+                const uint64_t qs = ct_two(qsum, qsum);
 #pragma unroll
                 for (int c = 0; c < 2; c++)
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         const float4 f = *reinterpret_cast<const float4 *>(ksc + c * 32 + i);
-                        s[c][i] = __float_as_uint(__uint_as_float(s[c][i]) * f.x);
-                        s[c][i + 1] = __float_as_uint(__uint_as_float(s[c][i + 1]) * f.y);
-                        s[c][i + 2] = __float_as_uint(__uint_as_float(s[c][i + 2]) * f.z);
-                        s[c][i + 3] = __float_as_uint(__uint_as_float(s[c][i + 3]) * f.w);
-                    }
-            } else if constexpr (NSC == 2) {
-#pragma unroll
-                for (int c = 0; c < 2; c++)
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float4 f = *reinterpret_cast<const float4 *>(ksc + (c * 32 + i) * 2);
-                        s[c][i] = __float_as_uint(fmaf(__uint_as_float(s[c][i]), f.x, qsum * f.y));
-                        s[c][i + 1] = __float_as_uint(fmaf(__uint_as_float(s[c][i + 1]), f.z, qsum * f.w));
+                        uint64_t u = ct_two(s[c][i], s[c][i + 1]), v = ct_two(s[c][i + 2], s[c][i + 3]);
+                        if constexpr (NSC == 2) {
+                            const float4 z = *reinterpret_cast<const float4 *>(ksc + CT_POS + c * 32 + i);
+                            u = ct_fma2(u, ct_two(f.x, f.y), ct_mul2(qs, ct_two(z.x, z.y)));
+                            v = ct_fma2(v, ct_two(f.z, f.w), ct_mul2(qs, ct_two(z.z, z.w)));
+                        } else {
+                            u = ct_mul2(u, ct_two(f.x, f.y));
+                            v = ct_mul2(v, ct_two(f.z, f.w));
+                        }
+                        s[c][i] = ct_first(u);
+                        s[c][i + 1] = ct_second(u);
+                        s[c][i + 2] = ct_first(v);
+                        s[c][i + 3] = ct_second(v);
                     }
             }
             if (p0 + 63 > all_to || !(p0 > all_low || (uint32_t)(p0 + 64) <= a.sinks)) {  // some row of the warp does not see all 64
@@ -637,13 +667,11 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                         if (!(see & (1u << i))) s[c][i] = 0xFF800000u;
                 }
             }
-            float mx[4];
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < 4; c++) mx[c] = __uint_as_float(s[c >> 1][(c & 1) * 16]);
+            for (int i = 0; i < 32; i += 4)
 #pragma unroll
-            for (int i = 1; i < 16; i++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) mx[c] = fmaxf(mx[c], __uint_as_float(s[c >> 1][(c & 1) * 16 + i]));
+                for (int c = 0; c < 4; c++) mx[c] = ct_max3(mx[c], s[c >> 1][i + (c & 1) * 2], s[c >> 1][i + (c & 1) * 2 + 1]);
             float best = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             best = fmaxf(best, other(best, j & 1));
             const float top = best == -INFINITY ? best : best * mul;  // mul may be 0
@@ -671,15 +699,16 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                 }
             }
             const float less = (m == -INFINITY ? 0.0f : m) - (BF16 ? 0.0f : CT_UP) - (CODES ? (float)max(ex - ref, -90) : 0.0f);
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const uint64_t mul2 = ct_two(mul, mul), less2 = ct_two(-less, -less);
+            uint64_t sum[2] = {0, 0};
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 uint32_t p[16];
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const float e0 = ct_ex2(fmaf(__uint_as_float(s[c][2 * i]), mul, -less)), e1 = ct_ex2(fmaf(__uint_as_float(s[c][2 * i + 1]), mul, -less));
-                    sum[(2 * i) & 3] += e0;
-                    sum[(2 * i + 1) & 3] += e1;
+                    const uint64_t x = ct_fma2(ct_two(s[c][2 * i], s[c][2 * i + 1]), mul2, less2);
+                    const float e0 = ct_ex2(__uint_as_float(ct_first(x))), e1 = ct_ex2(__uint_as_float(ct_second(x)));
+                    sum[i & 1] = ct_add2(sum[i & 1], ct_two(e0, e1));
                     if constexpr (BF16) {
                         const __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
                         p[i] = *reinterpret_cast<const uint32_t *>(&h);
@@ -690,7 +719,8 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                 }
                 t5::st16(s_col + half * 32 + c * 16, p);
             }
-            float more = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            sum[0] = ct_add2(sum[0], sum[1]);
+            float more = __uint_as_float(ct_first(sum[0])) + __uint_as_float(ct_second(sum[0]));
             if constexpr (CODES)
                 if (ex != ref) more *= ct_pow2(min(ref - ex, 90));
             l += more;
@@ -905,8 +935,8 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             for (int h = 0; h < 2; h++) {
                 const uint32_t row = ct + h * 96;
                 if (row < CT_POS) {
-                    if constexpr (NSC == 2) reinterpret_cast<float2 *>(ksc)[row] = scr[0][h];
-                    else ksc[row] = scr[0][h].x;
+                    ksc[row] = scr[0][h].x;
+                    if constexpr (NSC == 2) ksc[CT_POS + row] = scr[0][h].y;
                 }
                 // no value is larger; scales that are not finite count for nothing, their values stay what they are
                 const float most = KIND == KV_INT4 ? fmaf(8.0f, fabsf(scr[1][h].x), fabsf(scr[1][h].y)) : fabsf(scr[1][h].x) * (KIND == KV_INT8 ? 128.0f : 448.0f);
