@@ -50,8 +50,8 @@ struct CtCfg {
     static constexpr int NSC = (int)kv_scales<KIND>(), ROWB = HD * (int)kv_bits<KIND>() / 8;
     static constexpr int SLOT = NSC ? 2 * CT_POS * NSC * 4 + 16 : 0;                   // key scales, value scales, each converting warp's largest of the latter
     static constexpr int K_OFF = 2 * TILE, V_OFF = K_OFF + CT_ST * TILE, SC_OFF = V_OFF + CT_ST * TILE, BAR_OFF = SC_OFF + CT_SC * SLOT;
-    // barriers: kfull, kempty, vfull, vempty [2 each], sfull, pfull, ofull [2 each], qfull, scales [4]
-    static constexpr int STATE_OFF = BAR_OFF + 8 * (4 * CT_ST + 7 + CT_SC);
+    // barriers: kfull, kempty, vfull, vempty [2 each], sfull, pfull, ofull, qfull [2 each], scales [4]
+    static constexpr int STATE_OFF = BAR_OFF + 8 * (4 * CT_ST + 8 + CT_SC);
     static constexpr int X_OFF = STATE_OFF + 24;                                       // what the two threads of a row tell each other
     static constexpr int R_OFF = X_OFF + 2 * 2 * CT_ROWS * 4;                          // CacheRow of each row
     static constexpr int PRE_OFF = R_OFF + CT_ROWS * (int)sizeof(CacheRow);            // position tiles of the row tiles before each
@@ -128,6 +128,24 @@ __device__ __forceinline__ uint64_t ct_add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
     return d;
+}
+// 2^x of two numbers on the multiply-add pipe, where the special function unit is the bound: x = n + f with n the nearest whole number (1.5 * 2^23
+// added and taken off), 2^f by a polynomial of degree 4 fitted to the smallest relative error on [-1/2, 1/2] (2.6e-6), n added to the
+// exponent.  LOW: numbers to 2^-126 give 0, as the unit gives (bf16 holds 2^-126, and a value may be 2^127): all results are less by what the
+// polynomial makes of 2^-126.  Else they give 2^-126, of which fp16 keeps nothing.
+template <bool LOW>
+__device__ __forceinline__ uint64_t ct_exp2(uint64_t x) {
+    float a, b;  // a NaN stays one, and ends as an infinite weight
+    asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(a) : "f"(__uint_as_float(ct_first(x))), "f"(-126.0f));
+    asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(b) : "f"(__uint_as_float(ct_second(x))), "f"(-126.0f));
+    const uint64_t y = ct_two(a, b), t = ct_add2(y, ct_two(12582912.0f, 12582912.0f));
+    const uint64_t f = ct_fma2(ct_add2(t, ct_two(-12582912.0f, -12582912.0f)), ct_two(-1.0f, -1.0f), y);
+    uint64_t p = ct_fma2(ct_two(0.009570102207362652f, 0.009570102207362652f), f, ct_two(0.05591786280274391f, 0.05591786280274391f));
+    p = ct_fma2(p, f, ct_two(0.240247443318367f, 0.240247443318367f));
+    p = ct_fma2(p, f, ct_two(0.6931217908859253f, 0.6931217908859253f));
+    p = ct_fma2(p, f, ct_two(0.9999992847442627f, 0.9999992847442627f));
+    const uint64_t e = ct_two(ct_first(p) + (ct_first(t) << 23), ct_second(p) + (ct_second(t) << 23));
+    return LOW ? ct_add2(e, ct_two(0x807FFFF4u, 0x807FFFF4u)) : e;
 }
 __device__ __forceinline__ float ct_max3(float a, uint32_t b, uint32_t c) {
     float d;
@@ -257,6 +275,12 @@ __device__ __forceinline__ void ct_convert(uint32_t tile, uint32_t flip, const u
 
 // The results of a row tile's part that this thread's row has, half of the columns: stored, or left as a part, which the last block to arrive joins.
 // A function of its own: inlined into the loop over parts it took some 350 registers more than there are.
+// Where 16-byte piece c of a row of q lies.
+template <int HD>
+__device__ __forceinline__ uint8_t *ct_q_piece(uint8_t *sm, uint32_t q, uint32_t row, uint32_t c) {
+    return sm + q * CtCfg<KV_F16, HD>::TILE + (c >> 3) * CtCfg<KV_F16, HD>::PANEL + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+}
+
 template <int KIND, int HD>
 __device__ __noinline__ void ct_results(const CtDev &d, const CtSegment &g, uint8_t *sm, uint32_t o_col, uint32_t warp, uint32_t lane, uint32_t mine, float m,
                                         float l, int32_t ref) {
@@ -274,9 +298,11 @@ __device__ __noinline__ void ct_results(const CtDev &d, const CtSegment &g, uint
     };
     // ---- results, half of the columns a thread: O times 2^(ref - 13) where V was over a power of two, as the weights' sum is 2^12-fold ----
     const float unit = CODES ? ct_pow2(ref - 13) : 1.0f;
-    float inv = 1.0f / l, odd = l > 0.0f ? 0.0f : 1.0f;        // not 0 once an output was not finite
+    float inv = 1.0f / l, odd = l > 0.0f && m > -INFINITY ? 0.0f : 1.0f;  // not 0 once an output was not finite; a row without a maximum saw nothing, or only -inf
     const uint32_t rr = g.r0 + q * 128 + row;
-    uint16_t *dst = a.out + (size_t)(g.x.row0 + rr / a.group) * a.out_stride + (size_t)(g.kh * a.group + rr % a.group) * HD + half * (HD / 2);  // of rows that are there
+    // Half a row a thread, through where its half of q was: the products that read it are complete.
+    constexpr int W = HD / 16, AT = 32 / W;                        // 16-byte pieces of half a row; rows that a warp stores at once
+    uint16_t *dst = a.out + (size_t)(g.x.row0 + (there ? rr / a.group : 0)) * a.out_stride + (size_t)(g.kh * a.group + (there ? rr % a.group : 0)) * HD + half * (HD / 2);
     auto store = [&](int c, const float (&o)[32]) {            // 32 columns
         uint32_t w[16];
 #pragma unroll
@@ -285,9 +311,18 @@ __device__ __noinline__ void ct_results(const CtDev &d, const CtSegment &g, uint
             odd = fmaf(u, 0.0f, fmaf(v, 0.0f, odd));
             w[i] = kv_round2(u, v, a.c.rows_bf16);
         }
-        if (there)
 #pragma unroll
-            for (int i = 0; i < 4; i++) reinterpret_cast<uint4 *>(dst + c * 32)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        for (int i = 0; i < 4; i++) *reinterpret_cast<uint4 *>(ct_q_piece<HD>(sm, q, row, half * W + c * 4 + i)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    };
+    auto stored = [&]() {                                      // all columns
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+            const uint32_t r = i * AT + lane / W, at = row - lane + r;
+            const uint4 v = *reinterpret_cast<const uint4 *>(ct_q_piece<HD>(sm, q, at, half * W + lane % W));
+            uint16_t *to = reinterpret_cast<uint16_t *>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(dst), r));
+            if (q * 128 + at < g.here) reinterpret_cast<uint4 *>(to)[lane % W] = v;
+        }
     };
     bool done = g.whole;
     if (g.whole) {
@@ -306,6 +341,7 @@ __device__ __noinline__ void ct_results(const CtDev &d, const CtSegment &g, uint
             store(c, v);
             __syncwarp();                                      // the next TMEM read takes the whole warp
         }
+        stored();
     } else {
         constexpr size_t PART = cache_part_floats(CT_ROWS, HD);
         const size_t at = q * 128 + row, c_first = half * (HD / 8);  // groups of four columns
@@ -373,6 +409,7 @@ __device__ __noinline__ void ct_results(const CtDev &d, const CtSegment &g, uint
                     }
                     store(c, v);
                 }
+                stored();
             }
         }
     }
@@ -394,6 +431,9 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                                                                     const __grid_constant__ CUtensorMap vmap) {
     using C = CtCfg<KIND, HD>;
     constexpr bool CODES = KIND >= KV_INT8, BF16 = KIND == KV_BF16;
+    // of 8 pairs of exponentials, those on the multiply-add pipe (ct_exp2): a group of 28 of 128-wide heads, 2048 tokens over 6144 positions, 16-bit
+    // rows: none 344 us, 2 323 us, 4 356 us; int8, whose instructions are the bound already: none 513 us, 2 540 us
+    constexpr int POLY = CODES ? 0 : 2;
     constexpr int ST = CT_ST, NSC = C::NSC;
     const CacheAttnDev &a = d.a;
     extern __shared__ uint8_t ct_raw[];
@@ -402,7 +442,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
     pdl_launch_dependents();
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
     const uint32_t b_kfull = base + C::BAR_OFF, b_kempty = b_kfull + 8 * ST, b_vfull = b_kempty + 8 * ST, b_vempty = b_vfull + 8 * ST,
-                   b_sfull = b_vempty + 8 * ST, b_pfull = b_sfull + 16, b_ofull = b_pfull + 16, b_qfull = b_ofull + 16, b_sc = b_qfull + 8;
+                   b_sfull = b_vempty + 8 * ST, b_pfull = b_sfull + 16, b_ofull = b_pfull + 16, b_qfull = b_ofull + 16, b_sc = b_qfull + 16;
     volatile uint32_t *err_flag = reinterpret_cast<volatile uint32_t *>(smem + C::STATE_OFF);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::STATE_OFF + 8);
     if (tid == 0) {
@@ -410,8 +450,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             t5::mbar_init(b_kfull + 8 * s, CODES ? C::CONV : 1); t5::mbar_init(b_kempty + 8 * s, 1);
             t5::mbar_init(b_vfull + 8 * s, CODES ? C::CONV : 1); t5::mbar_init(b_vempty + 8 * s, 1);
         }
-        for (int q = 0; q < 2; q++) { t5::mbar_init(b_sfull + 8 * q, 1); t5::mbar_init(b_pfull + 8 * q, CT_SOFT / 2); t5::mbar_init(b_ofull + 8 * q, 1); }
-        t5::mbar_init(b_qfull, CT_SOFT);
+        for (int q = 0; q < 2; q++) { t5::mbar_init(b_sfull + 8 * q, 1); t5::mbar_init(b_pfull + 8 * q, CT_SOFT / 2); t5::mbar_init(b_ofull + 8 * q, 1); t5::mbar_init(b_qfull + 8 * q, CT_SOFT / 2); }
         for (int s = 0; s < CT_SC; s++) t5::mbar_init(b_sc + 8 * s, C::CONV);
         *err_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -573,24 +612,35 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         }
         float mul = fabsf(a.scale) * 1.4426950408889634f, qsum = 0.0f;
         {   // half of the row of q into its tile, its sign that of the scale
-            constexpr int W = HD / 16;
+            constexpr int W = HD / 16, AT = 32 / W;                // 16-byte pieces; rows that a warp fetches at once
             const uint32_t rr = g.r0 + q * 128 + row, token = there ? rr / a.group : 0, head = g.kh * a.group + (there ? rr % a.group : 0);
             const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-            const uint4 *src = reinterpret_cast<const uint4 *>(a.q + (size_t)(g.x.row0 + token) * a.q_stride + (size_t)head * HD) + half * W;
+            const uint16_t *src = a.q + (size_t)(g.x.row0 + token) * a.q_stride + (size_t)head * HD + half * (HD / 2);
             uint4 w[W];
-            float big = 0.0f;
 #pragma unroll
             for (int i = 0; i < W; i++) {
-                w[i] = there ? src[i] : make_uint4(0, 0, 0, 0);
+                const uint32_t r = i * AT + l_now / W;
+                const uint16_t *from = reinterpret_cast<const uint16_t *>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(src), r));
+                w[i] = q * 128 + row - l_now + r < g.here ? reinterpret_cast<const uint4 *>(from)[l_now % W] : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < W; i++) {
                 uint32_t *u = reinterpret_cast<uint32_t *>(&w[i]);
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    u[k] ^= flip;
-                    if constexpr (CODES)
-                        big = fmaxf(big, fmaxf(fabsf(kv_row_value((uint16_t)u[k], a.c.rows_bf16)), fabsf(kv_row_value((uint16_t)(u[k] >> 16), a.c.rows_bf16))));
-                }
+                for (int k = 0; k < 4; k++) u[k] ^= flip;
+                *reinterpret_cast<uint4 *>(ct_q_piece<HD>(sm, q, row - l_now + i * AT + l_now / W, half * W + l_now % W)) = w[i];
             }
             if constexpr (CODES) {                                 // over the power of two below the largest
+                __syncwarp();
+                float big = 0.0f;
+#pragma unroll
+                for (int i = 0; i < W; i++) {
+                    w[i] = *reinterpret_cast<const uint4 *>(ct_q_piece<HD>(sm, q, row, half * W + i));
+                    uint32_t *u = reinterpret_cast<uint32_t *>(&w[i]);
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        big = fmaxf(big, fmaxf(fabsf(kv_row_value((uint16_t)u[k], a.c.rows_bf16)), fabsf(kv_row_value((uint16_t)(u[k] >> 16), a.c.rows_bf16))));
+                }
                 big = fmaxf(big, other(big, 0));
                 const uint32_t ex = min(__float_as_uint(big) & 0x7F800000u, 253u << 23);
                 const float inv = ex ? __uint_as_float((254u << 23) - ex) : 1.0f;
@@ -607,15 +657,12 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                     }
                 }
                 if constexpr (NSC == 2) qsum += other(qsum, 1);
-            }
 #pragma unroll
-            for (int i = 0; i < W; i++) {
-                const uint32_t c = half * W + i;
-                *reinterpret_cast<uint4 *>(sm + q * C::TILE + (c >> 3) * C::PANEL + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = ct_order<KIND>(w[i]);
+                for (int i = 0; i < W; i++) *reinterpret_cast<uint4 *>(ct_q_piece<HD>(sm, q, row, half * W + i)) = ct_order<KIND>(w[i]);
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             asm volatile("bar.sync %0, 64;\n" ::"r"(1 + q * 4 + (w_now & 3)) : "memory");  // the exchanged values have been read
-            if (l_now == 0) t5::mbar_arrive(b_qfull);
+            if (l_now == 0) t5::mbar_arrive(b_qfull + 8 * q);
         }
         float m = -INFINITY, l = 0.0f;
         int32_t ref = 0;                                           // exponent that O is over
@@ -707,8 +754,11 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const uint64_t x = ct_fma2(ct_two(s[c][2 * i], s[c][2 * i + 1]), mul2, less2);
-                    const float e0 = ct_ex2(__uint_as_float(ct_first(x))), e1 = ct_ex2(__uint_as_float(ct_second(x)));
-                    sum[i & 1] = ct_add2(sum[i & 1], ct_two(e0, e1));
+                    uint64_t e;
+                    if (i % 8 < POLY) e = ct_exp2<BF16>(x);
+                    else e = ct_two(ct_ex2(__uint_as_float(ct_first(x))), ct_ex2(__uint_as_float(ct_second(x))));
+                    const float e0 = __uint_as_float(ct_first(e)), e1 = __uint_as_float(ct_second(e));
+                    sum[i & 1] = ct_add2(sum[i & 1], e);
                     if constexpr (BF16) {
                         const __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
                         p[i] = *reinterpret_cast<const uint32_t *>(&h);
@@ -757,15 +807,17 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             const CtSegment &g = segs[i];
             const uint32_t n = g.n, n_q = g.n_q, T = g.T, T1 = g.T1;
             if (n) {
-                t5::mbar_wait_bounded(b_qfull, g.Q & 1, err_flag);
                 t5::mbar_wait_bounded(b_kfull + 8 * (T % ST), (T / ST) & 1, err_flag);
-                __syncwarp();
-                t5::fence_after();
-                if (t5::elect_one()) {
-                    for (uint32_t q = 0; q < n_q; q++) scores(q, T);
-                    t5::commit(b_kempty + 8 * (T % ST));
+                for (uint32_t q = 0; q < n_q; q++) {
+                    t5::mbar_wait_bounded(b_qfull + 8 * q, g.Q & 1, err_flag);
+                    __syncwarp();
+                    t5::fence_after();
+                    if (t5::elect_one()) {
+                        scores(q, T);
+                        if (q + 1 == n_q) t5::commit(b_kempty + 8 * (T % ST));
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
             for (uint32_t j = 0; j < n; j++) {
                 const uint32_t J = T + j, st = J % ST, ph = (J / ST) & 1, va = base + C::V_OFF + st * C::TILE;
