@@ -16,8 +16,8 @@
 // Positions past the end are zero.  A position that some row of the block does not see meets weight 0, which an infinity there turns into
 // NaN: a row whose result is not finite is taken again by itself (cache_plain_row).
 //
-// Where there are fewer row tiles than SMs the positions are cut into S parts, whose maxima, sums and O go to scratch: up to CR_LAST of them
-// the last block to arrive joins in order, more than that cache_join_kernel.
+// Where there are few row tiles the positions are cut into S parts.  Up to eight are the blocks of a cluster, each of which joins some rows out of
+// the shared memory of all (through scratch and a counter: 14 heads of 64 over 711 positions 9.0 us, by clusters 5.5); more go through scratch to cache_join_kernel.
 // Bound: HBM for long caches (with 4-bit codes, the integer instructions of unpacking: some 1.2 a value), the latency of the chain (places,
 // tiles, joining) for short ones.
 #include <algorithm>
@@ -30,7 +30,13 @@
 namespace prism {
 
 constexpr int CR_W = 4, CR_THREADS = CR_W * 32;  // warps of a block
-constexpr uint32_t CR_LAST = 16;                 // parts that the last block joins
+constexpr uint32_t CR_CLUSTER = 8;               // parts whose blocks are a cluster
+constexpr uint32_t CR_NEAR = 512;                // positions of a part
+// More than 32 rows of a cached head are for the tcgen05 kernel, whose blocks cost 6 us more to begin and to end, where 16-row tiles are more than
+// two an SM or tiles times positions more than this.  8 cached heads of 128, 64 to 256 rows (int8): one sequence of 2000 positions 12 to 25 us here,
+// 20 to 24 there; eight of 711 20 to 75 here, 25 to 34 there; eight of 8000 149 to 559 here, 130 to 146 there.  To 32 rows this one always:
+// eight of 8000 positions, 32 rows: int8 71 us here, 128 there, 16 bits 68 and 75.
+constexpr uint64_t CR_WORK = 200000;
 constexpr float CR_UP = 16384.0f;                // weights of fp16 products of codes are 2^14-fold, and below 2; of fp16 rows 2^13-fold, and below 2^CR_GROW
 constexpr float CR_GROW = 2.0f;                  // powers of two that a score may lie above the maximum in use
 template <int KIND, int HD, int NQ>              // NQ: groups of eight query rows
@@ -48,7 +54,7 @@ struct CrCfg {
     static constexpr int BODY = RING > PARTS ? RING : PARTS;         // also the warps' parts of O and their sum
     static constexpr int Q_OFF = BODY, FRAG_OFF = Q_OFF + R * HD * 2;  // q rows, then as fragments
     static constexpr int ROW_OFF = FRAG_OFF + R * HD * 2;            // CrRow of each row, then maxima and sums: the warps', the row's; flags
-    static constexpr size_t SMEM = ROW_OFF + R * 32 + CR_W * R * 8 + R * 8 + (int)CR_LAST * R * 4 + 16;
+    static constexpr size_t SMEM = ROW_OFF + R * 32 + CR_W * R * 8 + R * 8 + 16;
     static constexpr int BLOCKS = HD <= 128 && NQ == 1 ? 3 : 2;      // of an SM, for the registers
 };
 struct CrRow {
@@ -63,7 +69,6 @@ struct CrDev {
     CacheAttnDev a;
     uint32_t splits, tiles;  // parts of the positions, row tiles of an entry and head
     float *part;             // of the blocks (CacheJoinDev)
-    unsigned int *count;     // [item], zero between launches
 };
 
 namespace {
@@ -160,6 +165,24 @@ __device__ __forceinline__ float cr_inv_pow2(float p) { return p > 0.0f ? __uint
 
 }  // namespace
 
+__device__ __forceinline__ void cr_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// From the same place of another block of the cluster.
+__device__ __forceinline__ float cr_lds_of(uint32_t at, uint32_t block) {
+    float v;
+    asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %1, %2;\nld.shared::cluster.f32 %0, [r];\n}\n" : "=f"(v) : "r"(at), "r"(block) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 cr_lds4_of(uint32_t at, uint32_t block) {
+    float4 v;
+    asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %4, %5;\nld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [r];\n}\n"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(at), "r"(block)
+                 : "memory");
+    return v;
+}
+
 template <int KIND, int HD, int NQ>
 __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache_rows_kernel(const __grid_constant__ CrDev d) {
     using C = CrCfg<KIND, HD, NQ>;
@@ -179,9 +202,8 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
     const uint32_t here = min((uint32_t)R, n_rows - r0), tok_lo = r0 / a.group, tok_hi = (r0 + here - 1) / a.group;
 
     CrRow *rows = reinterpret_cast<CrRow *>(cr_smem + C::ROW_OFF);
-    float *w_max = reinterpret_cast<float *>(cr_smem + C::ROW_OFF + R * 32), *w_sum = w_max + CR_W * R, *r_max = w_sum + CR_W * R, *r_sum = r_max + R,
-          *wgt = r_sum + R;
-    uint32_t *flags = reinterpret_cast<uint32_t *>(wgt + CR_LAST * R);  // rows to be taken again; whether this block joins
+    float *w_max = reinterpret_cast<float *>(cr_smem + C::ROW_OFF + R * 32), *w_sum = w_max + CR_W * R, *r_max = w_sum + CR_W * R, *r_sum = r_max + R;
+    uint32_t *flags = reinterpret_cast<uint32_t *>(r_sum + R);  // rows to be taken again
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(cr_smem) + warp * ST * C::STAGE;
 
     // ---- the positions that some row sees: the first tiles (a.sinks), then main_lo .. ---------------------------------
@@ -670,8 +692,8 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
     }
     __syncthreads();
 
-    // ---- the blocks' parts ---------------------------------------------------------------------------------------------------
-    if (d.splits > 1) {
+    // ---- the blocks' parts: left to cache_join_kernel, or each block joins some rows out of the shared memory of all -----------------------------
+    if (d.splits > CR_CLUSTER) {
         constexpr size_t PART = cache_part_floats(R, HD);
         float *mine = d.part + (size_t)blockIdx.x * PART;
         for (uint32_t i = tid; i < VALUES / 4; i += CR_THREADS)
@@ -680,54 +702,41 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
             __stcg(mine + VALUES + tid, r_max[tid]);
             __stcg(mine + VALUES + R + tid, r_sum[tid]);
         }
-        if (d.splits > CR_LAST) return;                    // cache_join_kernel follows
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-            const bool last = atomicAdd(d.count + item, 1u) == d.splits - 1;
-            if (last) d.count[item] = 0;                   // for the next launch
-            flags[1] = last;
-        }
-        __syncthreads();
-        if (!flags[1]) return;
-        __threadfence();
-        const float *all = d.part + (size_t)item * d.splits * PART;
-        if (tid < R) {
-            float top = -INFINITY, sum = 0.0f;
-#pragma unroll 8
-            for (uint32_t s = 0; s < d.splits; s++) top = fmaxf(top, __ldcg(all + s * PART + VALUES + tid));
-            const float sub = top == -INFINITY ? 0.0f : top;
-#pragma unroll 8
-            for (uint32_t s = 0; s < d.splits; s++) {
-                const float f = cr_ex2(__ldcg(all + s * PART + VALUES + tid) - sub);
-                wgt[s * R + tid] = f;
-                sum += __ldcg(all + s * PART + VALUES + R + tid) * f;
-            }
-            r_sum[tid] = sum;
-        }
-        __syncthreads();
-        for (uint32_t i = tid; i < VALUES / 4; i += CR_THREADS) {
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-            for (uint32_t s = 0; s < d.splits; s++) {
-                const float4 u = __ldcg(reinterpret_cast<const float4 *>(all + s * PART) + i);
-                const float f = wgt[s * R + i % R];
-                v.x = fmaf(u.x, f, v.x);
-                v.y = fmaf(u.y, f, v.y);
-                v.z = fmaf(u.z, f, v.z);
-                v.w = fmaf(u.w, f, v.w);
-            }
-            *reinterpret_cast<float4 *>(acc + i % R * PITCH + i / R * 4) = v;
-        }
-        __syncthreads();
+        return;
     }
+    const uint32_t lo = split * R / d.splits, hi = min((split + 1) * R / d.splits, here);  // rows of this block
+    if (d.splits > 1) cr_cluster_sync();
 
     // ---- results: four columns of a row a thread ------------------------------------------------------------------------------
-    for (uint32_t u = tid; u < VALUES / 4; u += CR_THREADS) {
-        const uint32_t r = u / (HD / 4), c = u % (HD / 4) * 4;
-        if (r >= here) continue;
-        const float sum = r_sum[r], inv = 1.0f / sum;
+    for (uint32_t u = tid; u < (hi > lo ? hi - lo : 0) * (HD / 4); u += CR_THREADS) {
+        const uint32_t r = lo + u / (HD / 4), c = u % (HD / 4) * 4;
+        float sum = r_sum[r];
         float4 v = *reinterpret_cast<const float4 *>(acc + r * PITCH + c);
+        if (d.splits > 1) {
+            const uint32_t max_at = (uint32_t)__cvta_generic_to_shared(r_max + r), sum_at = (uint32_t)__cvta_generic_to_shared(r_sum + r),
+                           acc_at = (uint32_t)__cvta_generic_to_shared(acc + r * PITCH + c);
+            float f[CR_CLUSTER], part[CR_CLUSTER], top = -INFINITY;
+            float4 w[CR_CLUSTER];
+#pragma unroll
+            for (uint32_t s = 0; s < CR_CLUSTER; s++) {
+                const uint32_t from = s < d.splits ? s : 0;
+                f[s] = cr_lds_of(max_at, from);
+                part[s] = cr_lds_of(sum_at, from);
+                w[s] = cr_lds4_of(acc_at, from);
+                if (s < d.splits) top = fmaxf(top, f[s]);
+            }
+            const float sub = top == -INFINITY ? 0.0f : top;
+            sum = 0.0f;
+            v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (uint32_t s = 0; s < CR_CLUSTER; s++)
+                if (s < d.splits) {
+                    const float k = cr_ex2(f[s] - sub);
+                    sum = fmaf(part[s], k, sum);
+                    v = make_float4(fmaf(w[s].x, k, v.x), fmaf(w[s].y, k, v.y), fmaf(w[s].z, k, v.z), fmaf(w[s].w, k, v.w));
+                }
+        }
+        const float inv = 1.0f / sum;
         v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
         if (!(sum > 0.0f) || !isfinite(v.x) || !isfinite(v.y) || !isfinite(v.z) || !isfinite(v.w)) {
             atomicOr(flags, 1u << r);
@@ -741,6 +750,7 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
     const uint32_t again = flags[0];
     for (uint32_t r = warp; r < here; r += CR_W)
         if (again >> r & 1) cache_plain_row<KIND, HD>(a, x, (r0 + r) / a.group, kh * a.group + (r0 + r) % a.group, lane);
+    if (d.splits > 1) cr_cluster_sync();                   // nobody leaves before the others have read its part
 }
 
 // ---- scratch -----------------------------------------------------------------------------------------------------------------
@@ -810,27 +820,61 @@ int cache_scratch(prism_cuda_ctx *ctx, size_t part_bytes, size_t counts, float *
 template <int KIND, int HD, int NQ>
 static int launch_rows_kernel(prism_cuda_ctx *ctx, const CacheAttnDev &a, uint32_t max_length) {
     using C = CrCfg<KIND, HD, NQ>;
-    static int resident[PRISM_MAX_DEVICES] = {0};          // blocks of an SM; 0: not asked yet
-    if (!resident[ctx->device]) {
+    static int room[PRISM_MAX_DEVICES][CR_CLUSTER + 1] = {{0}};  // clusters of that many blocks that the device holds at once; [0]: asked already
+    if (!room[ctx->device][0]) {
         PRISM_CUDA_TRY(ctx, cudaFuncSetAttribute(cache_rows_kernel<KIND, HD, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
         int n = 0;
         PRISM_CUDA_TRY(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, cache_rows_kernel<KIND, HD, NQ>, CR_THREADS, C::SMEM));
         if (n < 1) return fail(ctx, PRISM_E_CUDA, "cache_rows_kernel does not fit an SM");
-        resident[ctx->device] = n;
+        room[ctx->device][1] = n * ctx->sm_count;
+        for (uint32_t size = 2; size <= CR_CLUSTER; size++) {
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(size);
+            cfg.blockDim = dim3(CR_THREADS);
+            cfg.dynamicSmemBytes = C::SMEM;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = size;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            PRISM_CUDA_TRY(ctx, cudaOccupancyMaxActiveClusters(&room[ctx->device][size], cache_rows_kernel<KIND, HD, NQ>, &cfg));
+        }
+        room[ctx->device][0] = 1;
     }
     CrDev d{};
     d.a = a;
     d.tiles = (uint32_t)(((uint64_t)a.max_tokens * a.group + C::R - 1) / C::R);
-    const uint64_t items = (uint64_t)a.n_entries * a.c.kv_heads * d.tiles, slots = (uint64_t)ctx->sm_count * resident[ctx->device];
+    const uint64_t items = (uint64_t)a.n_entries * a.c.kv_heads * d.tiles, slots = (uint64_t)room[ctx->device][1];
     uint64_t seen = max_length;
     if (a.window) seen = std::min<uint64_t>(seen, (uint64_t)a.window + a.sinks + 2 * C::TP);
     const uint64_t most = (seen + C::TP * CR_W - 1) / (C::TP * CR_W);  // parts in which every warp has a tile
-    d.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(most, CJ_MAX_SPLIT), slots / items));
-    if (items * d.splits > 0x7FFFFFFFull) return fail(ctx, PRISM_E_ARG, "cache_attention: too many rows");
-    if (d.splits > 1) PRISM_TRY(cache_scratch(ctx, (size_t)(items * d.splits) * cache_part_floats(C::R, HD) * 4, (size_t)items, &d.part, &d.count));
-    launch_pdl(ctx, "cache_rows_kernel", cache_rows_kernel<KIND, HD, NQ>, dim3((uint32_t)(items * d.splits)), dim3(CR_THREADS), C::SMEM, d);
+    // Parts that fill the GPU once, where they are more than a cluster: a cluster joins in a microsecond, scratch and a second kernel in four, which
+    // is worth it where a block of a cluster had more than CR_NEAR positions (8 heads of 128, 24 drafts of 8000 positions: 22 us by clusters, 18 by
+    // parts; 6000 positions of one sequence: 13.1 and 12.6; 2000: 8.4 and 10.4).
+    uint64_t parts = std::min<uint64_t>(std::min<uint64_t>(most, CJ_MAX_SPLIT), slots / items);
+    if (parts <= CR_CLUSTER || seen <= CR_CLUSTER * CR_NEAR) {
+        // Else the size of cluster with the smallest waves * (positions of a part + what a block costs besides, in positions).  A block costs 6 us:
+        // 650 positions of 128 codes; 16-bit rows are bound by HBM from half of the blocks on, and lose more by a second wave.  256 row tiles of
+        // 128-wide heads, one part and three: int8 over 8000 positions 113 and 76 us, over 2000 38 and 33; 16 bits 124 and 103, 38 and 37.
+        constexpr uint64_t BESIDE = KIND >= KV_INT8 ? 650 : 2000;
+        uint64_t least = UINT64_MAX;
+        for (uint32_t size = 1; size <= CR_CLUSTER && size <= std::max<uint64_t>(most, 1); size++) {
+            const uint64_t at_once = (uint64_t)std::max(room[ctx->device][size], 1);
+            const uint64_t cost = (items + at_once - 1) / at_once * ((seen + size - 1) / size + BESIDE);
+            if (cost < least) {
+                least = cost;
+                parts = size;
+            }
+        }
+    }
+    d.splits = (uint32_t)parts;
+    if (items * parts > 0x7FFFFFFFull) return fail(ctx, PRISM_E_ARG, "cache_attention: too many rows");
+    const bool join = parts > CR_CLUSTER;
+    if (join) PRISM_TRY(cache_scratch(ctx, (size_t)(items * parts) * cache_part_floats(C::R, HD) * 4, 0, &d.part, nullptr));
+    launch_cluster_pdl(ctx, cache_rows_kernel<KIND, HD, NQ>, dim3((uint32_t)(items * parts)), dim3(CR_THREADS), C::SMEM, join ? 1u : (unsigned)parts, d);
     PRISM_TRY(after_launch(ctx, "cache_rows_kernel"));
-    return d.splits > CR_LAST ? launch_cache_join<KIND, HD>(ctx, CacheJoinDev{a, d.splits, d.tiles, (uint32_t)C::R, d.part}) : PRISM_OK;
+    return join ? launch_cache_join<KIND, HD>(ctx, CacheJoinDev{a, d.splits, d.tiles, (uint32_t)C::R, d.part}) : PRISM_OK;
 }
 
 template <int KIND>
@@ -885,7 +929,10 @@ static int cache_attention(prism_cuda_ctx *ctx, const prism_cache *c, const pris
     a.tree = p->tree;
     a.tree_words = p->tree_words;
     a.q_pos = p->q_pos;
-    if ((uint64_t)a.max_tokens * a.group > 16 && cache_tiles_fit(a, c->head_dim)) return launch_cache_tiles(ctx, kind, c->head_dim, a, p->max_length);
+    const uint64_t rows = (uint64_t)a.max_tokens * a.group, seen = a.window ? std::min<uint64_t>(p->max_length, (uint64_t)a.window + a.sinks) : p->max_length;
+    const uint64_t items = (rows + 15) / 16 * a.n_entries * c->kv_heads;
+    if (rows > 32 && (items > 2 * (uint64_t)ctx->sm_count || items * seen > CR_WORK) && cache_tiles_fit(a, c->head_dim))
+        return launch_cache_tiles(ctx, kind, c->head_dim, a, p->max_length);
     switch (kind) {
     case KV_F16: return launch_kind<KV_F16>(ctx, c->head_dim, a, p->max_length);
     case KV_BF16: return launch_kind<KV_BF16>(ctx, c->head_dim, a, p->max_length);
