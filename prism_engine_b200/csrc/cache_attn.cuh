@@ -69,8 +69,8 @@ __device__ __forceinline__ bool cache_sees(const CacheAttnDev &a, const CacheEnt
     return c <= r.last && (c > r.low || (uint32_t)c < a.sinks);
 }
 
-// One token's output for one head by one warp in 32 bits, position by position, in two passes: the largest score, then the weights
-// and the sums.  What the formula gives for infinities and NaN is what this gives; positions that the row does not see take no part.
+// One token's output for one head by one warp in 32 bits, position by position, in three passes: the largest score, the sum of the weights, the
+// values over that sum, which is no larger than the largest of them (values near bf16's largest overflow the sums of the other kernels).  What the formula gives for infinities and NaN is what this gives; positions that the row does not see take no part.
 template <int KIND, int HD>
 __device__ __noinline__ void cache_plain_row(const CacheAttnDev &a, const CacheEntry &x, uint32_t token, uint32_t head, uint32_t lane) {
     constexpr int VEC = HD / 32;
@@ -85,7 +85,7 @@ __device__ __noinline__ void cache_plain_row(const CacheAttnDev &a, const CacheE
     }
     float top = -INFINITY, sum = 0.0f;
     bool any = false;
-    for (int pass = 0; pass < 2; pass++) {
+    for (int pass = 0; pass < 3; pass++) {
         // positions that no row under this window sees are stepped over
         const int32_t gap_lo = (int32_t)min(a.sinks, 0x7FFFFFFFu), gap_hi = min(r.low, x.first - 1);
         for (int32_t p = 0; p < x.len; p++) {
@@ -106,9 +106,10 @@ __device__ __noinline__ void cache_plain_row(const CacheAttnDev &a, const CacheE
             any = true;
             if (pass == 0) {
                 top = fmaxf(top, d);
+            } else if (pass == 1) {
+                sum += expf(d - top);
             } else {
-                const float w = expf(d - top);
-                sum += w;
+                const float w = expf(d - top) / sum;
                 kv_values<KIND, VEC>(a.c.v + at * ROWB, a.c.vs + at * kv_scales<KIND>(), col, v);
 #pragma unroll
                 for (int i = 0; i < VEC; i++) acc[i] = fmaf(w, v[i], acc[i]);
@@ -117,7 +118,7 @@ __device__ __noinline__ void cache_plain_row(const CacheAttnDev &a, const CacheE
     }
     uint16_t *dst = a.out + (size_t)(x.row0 + token) * a.out_stride + (size_t)head * HD + col;
 #pragma unroll
-    for (int i = 0; i < VEC; i++) dst[i] = kv_round(any ? acc[i] / sum : 0.0f, a.c.rows_bf16);
+    for (int i = 0; i < VEC; i++) dst[i] = kv_round(any ? acc[i] : 0.0f, a.c.rows_bf16);
 }
 #endif
 
