@@ -341,7 +341,7 @@ int prism_cuda_cache_keep_dev(prism_cuda_ctx *ctx, const prism_cache *cache, uin
  * bits; a row that sees nothing is 0, rows of no entry (and of an entry with a negative sequence) are left as they were. */
 typedef struct prism_cache_attention {
     const void *q;           /* rows of num_heads * head_dim values */
-    void *out;
+    void *out;               /* overlaps neither q nor the cache */
     uint64_t q_stride, out_stride;  /* values between rows, multiples of 8 */
     uint32_t n_rows;         /* rows of q and out */
     uint32_t n_entries;

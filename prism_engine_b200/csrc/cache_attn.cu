@@ -18,8 +18,10 @@
 //
 // Where there are few row tiles the positions are cut into S parts.  Up to eight are the blocks of a cluster, each of which joins some rows out of
 // the shared memory of all (through scratch and a counter: 14 heads of 64 over 711 positions 9.0 us, by clusters 5.5); more go through scratch to cache_join_kernel.
-// Bound: HBM for long caches (with 4-bit codes, the integer instructions of unpacking: some 1.2 a value), the latency of the chain (places,
-// tiles, joining) for short ones.
+// Bound: HBM for long caches of 16-bit rows; the instructions about codes (some 850 a warp for 32 positions of a 128-wide head: places, copies, bytes to
+// fragments, scales, softmax) at 8 and 4 bits; the latency of the chain (places, tiles, joining) for short ones.
+// 64 heads of 128 over 8, a token of 32 sequences under a window of 4096: 16 bits 85 us (6.3 TB/s), int8 63 us (4.4 TB/s), int4 64 us; one sequence of 131071
+// positions: 16 bits 93 us (5.8 TB/s), int4 56 us (2.7 TB/s); 14 heads of 64 over 2, 516 visible positions: 5.5 us.
 #include <algorithm>
 #include <cmath>
 #include <stdexcept>
@@ -909,6 +911,7 @@ static int cache_attention(prism_cuda_ctx *ctx, const prism_cache *c, const pris
         ((reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->out)) & 15))
         return fail(ctx, PRISM_E_ARG, "cache_attention: rows must be 16-byte aligned and at least num_heads * head_dim values apart");
     if (reinterpret_cast<uintptr_t>(p->tree) & 7) return fail(ctx, PRISM_E_ARG, "cache_attention: masks must be 8-byte aligned");
+    if (p->q == p->out) return fail(ctx, PRISM_E_ARG, "cache_attention: results must not overlap the queries");  // a row may be taken again
     DeviceGuard on(ctx->device);
     if (on.err != cudaSuccess) return cuda_fail(ctx, on.err, "cudaSetDevice");
     a.q = static_cast<const uint16_t *>(p->q);

@@ -243,3 +243,15 @@ def test_oracle_agrees_with_the_row_by_row_one():
     for kw in (dict(), dict(window=9, sinks=2), dict(masks=[0, 1, 3, 5, 9] + [j * 5 for j in range(7)], q_pos=list(range(12)), window=6, sinks=1)):
         for got, want in zip(oracle(c, q, entries, 4, **kw), attention(c, q, entries, 4, **kw)):
             assert torch.allclose(got, want, rtol=1e-6 if got is not None else 0, atol=1e-4)
+
+
+def test_results_over_the_queries_are_refused(backend):
+    from prism_engine_b200 import PrismCudaError
+
+    c = Cache("int8", "fp16", 2, 64, n_seqs=1, max_len=32, page=16)
+    x, s = torch.zeros(4, 4, 64, dtype=torch.float16, device="cuda"), i32([0, 4, 4])
+    torch.cuda.synchronize()
+    with pytest.raises(PrismCudaError, match="overlap") as e:
+        backend.cache_attention_dev(c.view(), q=x.data_ptr(), out=x.data_ptr(), n_rows=4, n_entries=1, seq=s.data_ptr(), q_start=s.data_ptr(),
+                                    length=s.data_ptr() + 4, max_tokens=4, max_length=4, num_heads=4)
+    assert e.value.code == -2
