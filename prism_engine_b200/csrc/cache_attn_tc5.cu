@@ -44,8 +44,8 @@ struct CtSegment {
     uint32_t whole;                       // the whole row tile
     uint32_t units, from, take;           // of the row tile, of this part
     uint32_t b0, b1, slot, slot0;         // blocks that have parts of the item; places of this block's part and of b0's
-    // barriers go on from part to part: position tiles before this one (T1: with a second tile of rows), parts with such tiles, with rows
-    uint32_t T, T1, S0, S1, Q;
+    // barriers go on from part to part: position tiles before this one (T1: with a second tile of rows), parts with such tiles
+    uint32_t T, T1, S0, S1;
 };
 template <int KIND, int HD>
 struct CtCfg {
@@ -561,19 +561,17 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         }
         __syncthreads();
         if (tid == 0) {
-            uint32_t T = 0, T1 = 0, S0 = 0, S1 = 0, Q = 0;
+            uint32_t T = 0, T1 = 0, S0 = 0, S1 = 0;
             for (uint32_t k = 0; k < pre[CT_PAIRS + 1]; k++) {
                 CtSegment &g = segs[k];
                 g.T = T;
                 g.T1 = T1;
                 g.S0 = S0;
                 g.S1 = S1;
-                g.Q = Q;
                 T += g.n;
                 T1 += g.n_q == 2 ? g.n : 0;
                 S0 += g.n > 0;
                 S1 += g.n > 0 && g.n_q == 2;
-                Q += g.here > 0;
             }
             pre[CT_PAIRS + 2] = T;
         }
@@ -605,6 +603,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         const CtSegment &g = *(reinterpret_cast<const CtSegment *>(sm + C::SEG_OFF) + k);
         if (g.here == 0) continue;
         const bool there = q * 128 + row < g.here;
+        const uint32_t mine = q < g.n_q ? g.n : 0, T = g.T, Tq = q ? g.T1 : T;
         int32_t all_to, all_low;
         {
             CacheRow r{0x7FFFFFF0, -1, nullptr};                   // a row that is not there: sees everything, is not stored
@@ -665,11 +664,11 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             asm volatile("bar.sync %0, 64;\n" ::"r"(1 + q * 4 + (w_now & 3)) : "memory");  // the exchanged values have been read
-            if (l_now == 0) t5::mbar_arrive(b_qfull + 8 * q);
+            // A phase only where the issuer waits for it: a wait tells a phase from the next by its parity alone, so no warp may be two ahead.
+            if (l_now == 0 && mine) t5::mbar_arrive(b_qfull + 8 * q);
         }
         float m = -INFINITY, l = 0.0f;
         int32_t ref = 0;                                           // exponent that O is over
-        const uint32_t mine = q < g.n_q ? g.n : 0, T = g.T, Tq = q ? g.T1 : T;
         for (uint32_t j = 0; j < mine; j++) {
             int32_t ex = 0;
             const float *ksc = nullptr;
@@ -812,7 +811,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             if (n) {
                 t5::mbar_wait_bounded(b_kfull + 8 * (T % ST), (T / ST) & 1, err_flag);
                 for (uint32_t q = 0; q < n_q; q++) {
-                    t5::mbar_wait_bounded(b_qfull + 8 * q, g.Q & 1, err_flag);
+                    t5::mbar_wait_bounded(b_qfull + 8 * q, (q ? g.S1 : g.S0) & 1, err_flag);
                     __syncwarp();
                     t5::fence_after();
                     if (t5::elect_one()) {

@@ -1,0 +1,87 @@
+"""Batches of single tokens, prompts and empty sequences whose work the blocks of the many-row attention share: sequences of parts in
+one block after which a hand-over could be taken for the one before it (a barrier's wait knows only a phase's parity).
+
+Bound per output as in test_gpu_cache_many_rows."""
+import math
+
+import pytest
+import torch
+
+from cache_parts import parts
+from cache_util import Cache, check, queries, run_attention
+from test_gpu_cache_many_rows import _both, _entries, oracle
+
+SMS = 148  # blocks that share the work
+two = lambda p: p[3] > 128 and p[4] > 0       # noqa: E731  both tiles of 128 rows, position tiles
+one = lambda p: 0 < p[3] <= 128 and p[4] > 0  # noqa: E731  the first tile of 128 rows only
+none = lambda p: p[3] > 0 and p[4] == 0       # noqa: E731  rows that see nothing
+
+
+def blocks_with(sizes, heads, kvh, *kinds, whole=True, **kw):
+    """How many blocks have parts of these kinds one after the other, whole row tiles all but the last."""
+    n = 0
+    for mine in parts(sizes, heads, kvh, SMS, **kw):
+        for i in range(len(mine) - len(kinds) + 1):
+            if all(k(p) and (p[5] or j + 1 == len(kinds) or not whole) for j, (k, p) in enumerate(zip(kinds, mine[i:]))):
+                n += 1
+                break
+    return n
+
+
+# ---- parts of 256, of at most 128, and of 256 rows ------------------------------------------------------------------------
+HALVES = [(32, 200 - i % 20) if i % 2 == 0 else (9 + i % 8, 190) for i in range(500)]  # 8 heads over one: 256 rows, then 72 to 128
+# ---- rows that see nothing among others --------------------------------------------------------------------------------------
+EMPTY = [(64, 300 + i) if i % 2 == 0 else (64, 0) for i in range(120)]
+EARLY = [(300, 20) if i % 2 == 0 else (64, 400) for i in range(60)]  # more tokens than positions: their first rows lie before position 0
+
+TURNS = [(32, 100) if i % 2 == 0 else (32, 0) for i in range(500)]
+
+
+def test_the_batches_have_such_blocks():
+    assert blocks_with(HALVES, 8, 1, two, one, two) == 102
+    assert blocks_with(EMPTY, 8, 1, none, two) == 43
+    assert blocks_with(EARLY, 8, 1, none, two) == 20
+    assert blocks_with(TURNS, 8, 1, two, none, two) == 102
+
+
+KINDS16 = [("16", "fp16", 128), ("16", "bf16", 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,rows,hd", KINDS16)
+def test_rows_taken_again_before_parts_of_one_and_two_tiles(backend, fmt, rows, hd):
+    """An infinite value that only the last token of every fourth entry sees: its other 248 rows are taken again, 102 blocks having a part
+    of at most 128 rows and one of 256 behind them."""
+    c = Cache(fmt, rows, 1, hd, n_seqs=20, max_len=200, page=16, seed=hd)
+    seqs = [i % 20 for i in range(len(HALVES))]
+    entries, n = _entries(HALVES, seqs)
+    q = queries(n, 8, hd, rows, 1)
+    want, tol = oracle(c, q, entries, 8)
+    odd = torch.zeros(n, dtype=torch.bool)
+    spoiled = {}
+    for s, r0, t, length in entries[::4]:
+        spoiled.setdefault(s, set()).add(length - 1)
+    for s, at in spoiled.items():
+        for p in at:
+            page, place = c.place(s, p)
+            c.pool["v"][page, 0, place, 5] = math.inf
+    for s, r0, t, length in entries:
+        for i in range(t):
+            odd[r0 + i] = any(p <= length - t + i for p in spoiled.get(s, ()))
+    got = run_attention(backend, c, q, entries, 8)
+    assert odd.any() and not odd.all()
+    check(got, want, tol, ~odd)
+    assert not torch.isfinite(got[odd][:, :, 5]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", [EMPTY, EARLY, TURNS], ids=["empty", "early", "turns"])
+@pytest.mark.parametrize("fmt,rows,hd", KINDS16)
+def test_rows_that_see_nothing_among_others(backend, fmt, rows, hd, sizes):
+    c = Cache(fmt, rows, 1, hd, n_seqs=20, max_len=430, page=32, seed=hd + 1)
+    got, again = _both(backend, c, sizes, 8, seqs=[i % 20 for i in range(len(sizes))], seed=2)
+    row = 0
+    for n, length in sizes:
+        assert (got[row:row + max(0, n - length)] == 0).all()
+        row += n
+    assert torch.equal(got, again())
