@@ -672,13 +672,15 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         for (uint32_t j = 0; j < mine; j++) {
             int32_t ex = 0;
             const float *ksc = nullptr;
+            t5::mbar_wait_warp(b_sfull + 8 * q, (Tq + j) & 1, err_flag);
             if constexpr (CODES) {
+                // After the scores, which follow these scales: before them a warp that had no rows in the parts before could be phases ahead of
+                // the slot, and parity would let it read an older tile's.  The wait passes at once, and makes the scales visible.
                 t5::mbar_wait_warp(b_sc + 8 * ((T + j) % CT_SC), ((T + j) / CT_SC) & 1, err_flag);
                 ksc = reinterpret_cast<const float *>(sm + C::SC_OFF + ((T + j) % CT_SC) * C::SLOT);
                 ex = ct_exponent(ksc + 2 * CT_POS * NSC);
                 ksc += half * 64;                                  // scales of all positions, then zeros
             }
-            t5::mbar_wait_warp(b_sfull + 8 * q, (Tq + j) & 1, err_flag);
             t5::fence_after();
             uint32_t s[2][32];
 #pragma unroll

@@ -36,12 +36,23 @@ EARLY = [(300, 20) if i % 2 == 0 else (64, 400) for i in range(60)]  # more toke
 
 TURNS = [(32, 100) if i % 2 == 0 else (32, 0) for i in range(500)]
 
+# ---- single tokens and a prompt ----------------------------------------------------------------------------------------------
+MIXED = [[(1, 1500)] * 7 + [(512, 2000)], [(1, 1500)] * 9 + [(256, 3000)]]
+
+
+def ahead(sizes, heads, kvh):
+    """Blocks in which a part of 256 rows follows a whole row tile of at most 128, four position tiles or more before it."""
+    return sum(any(one(p) and p[5] and two(mine[i + 1]) and sum(x[4] for x in mine[:i + 1]) >= 4 for i, p in enumerate(mine[:-1]))
+               for mine in parts(sizes, heads, kvh, SMS))
+
 
 def test_the_batches_have_such_blocks():
     assert blocks_with(HALVES, 8, 1, two, one, two) == 102
     assert blocks_with(EMPTY, 8, 1, none, two) == 43
     assert blocks_with(EARLY, 8, 1, none, two) == 20
     assert blocks_with(TURNS, 8, 1, two, none, two) == 102
+    for sizes in MIXED:
+        assert ahead(sizes, 64, 8) > 0
 
 
 KINDS16 = [("16", "fp16", 128), ("16", "bf16", 64)]
@@ -85,3 +96,26 @@ def test_rows_that_see_nothing_among_others(backend, fmt, rows, hd, sizes):
         assert (got[row:row + max(0, n - length)] == 0).all()
         row += n
     assert torch.equal(got, again())
+
+
+CODED = [("int8", "fp16", 128), ("e4m3", "bf16", 128), ("int4", "bf16", 128), ("int8", "bf16", 64), ("int4", "fp16", 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", MIXED, ids=["seven", "nine"])
+@pytest.mark.parametrize("fmt,rows,hd", CODED)
+def test_single_tokens_and_a_prompt_over_codes(backend, fmt, rows, hd, sizes):
+    """The values of neighbouring sequences differ 2^6-fold, so that another tile's exponent of the values would show."""
+    c = Cache(fmt, rows, 8, hd, n_seqs=len(sizes), max_len=max(x for _, x in sizes), page=64, seed=hd + 2)
+    for s in range(len(sizes)):
+        c.scale["v"][c.table_cpu[s].long().cuda()] *= 2.0 ** (3 if s % 2 else -3)
+    _both(backend, c, sizes, 64, seed=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,rows,hd", CODED)
+def test_turns_of_rows_over_codes(backend, fmt, rows, hd):
+    """The batches above over codes."""
+    for sizes in (HALVES, EMPTY, EARLY, TURNS):
+        c = Cache(fmt, rows, 1, hd, n_seqs=20, max_len=430, page=32, seed=hd + 3)
+        _both(backend, c, sizes, 8, seqs=[i % 20 for i in range(len(sizes))], seed=4)
