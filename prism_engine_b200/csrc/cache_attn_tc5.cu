@@ -13,7 +13,7 @@
 //                 by the exponent in which its tile lies below the largest so far.  A value 2^27 below the largest of its tile loses bits.
 //
 // Positions past the end are zero.  A position that a row does not see meets weight 0, which an infinity there turns into NaN: a row whose
-// result is not finite is taken again by itself (cache_plain_row).
+// result is not finite is taken again by itself (cache_plain_row), after all parts of its block.
 // Few row tiles: the positions are cut into parts whose fp32 sums cache_join_kernel joins in order.  More of them: the blocks, one an SM, share
 // all tiles of positions evenly, whatever the lengths, and copies and conversions of a row tile begin under the results of the one before.
 // Bound: the tensor core and the instructions about the scores together: 2 048 cycles of products for 256 rows and 128 positions of a 128-wide head,
@@ -46,6 +46,7 @@ struct CtSegment {
     uint32_t b0, b1, slot, slot0;         // blocks that have parts of the item; places of this block's part and of b0's
     // barriers go on from part to part: position tiles before this one (T1: with a second tile of rows), parts with such tiles
     uint32_t T, T1, S0, S1;
+    uint32_t again[CT_ROWS / 32];         // rows to be taken again by themselves: a bit each
 };
 template <int KIND, int HD>
 struct CtCfg {
@@ -285,7 +286,7 @@ __device__ __forceinline__ uint8_t *ct_q_piece(uint8_t *sm, uint32_t q, uint32_t
 }
 
 template <int KIND, int HD>
-__device__ __noinline__ void ct_results(const CtDev &d, const CtSegment &g, uint8_t *sm, uint32_t o_col, uint32_t warp, uint32_t lane, uint32_t mine, float m,
+__device__ __noinline__ void ct_results(const CtDev &d, CtSegment &g, uint8_t *sm, uint32_t o_col, uint32_t warp, uint32_t lane, uint32_t mine, float m,
                                         float l, int32_t ref) {
     using C = CtCfg<KIND, HD>;
     constexpr bool CODES = KIND >= KV_INT8;
@@ -417,14 +418,8 @@ __device__ __noinline__ void ct_results(const CtDev &d, const CtSegment &g, uint
         }
     }
     const float theirs = other(odd, (mine & 1) ^ 1);           // every lane takes part; after what the other thread stored
-    if (done) {
-        const bool again = there && (odd != 0.0f || theirs != 0.0f);
-        if (half == 0)
-            for (uint32_t rows = __ballot_sync(0xFFFFFFFFu, again); rows; rows &= rows - 1) {
-                const uint32_t i = rr - lane + (uint32_t)(__ffs(rows) - 1);
-                cache_plain_row<KIND, HD>(a, g.x, i / a.group, g.kh * a.group + i % a.group, lane);
-            }
-    }
+    const uint32_t again = __ballot_sync(0xFFFFFFFFu, done && there && (odd != 0.0f || theirs != 0.0f));
+    if (half == 0 && lane == 0) g.again[q * 4 + (warp & 3)] = again;
 }
 
 }  // namespace
@@ -548,6 +543,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             CacheEntry x{};
             CtTiles t{};
             if (cache_entry(a, pair / d.tiles, x)) t = ct_tiles<true>(a, x, pair % d.tiles);  // the same in all blocks of an item
+            if (lane < CT_ROWS / 32) g.again[lane] = 0;
             if (lane == 0) {
                 g.x = x;
                 g.r0 = pair % d.tiles * CT_ROWS;
@@ -600,7 +596,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             return xch[(turn * 2 + (half ^ 1)) * CT_ROWS];
         };
         CacheRow *row_at = reinterpret_cast<CacheRow *>(sm + C::R_OFF) + q * 128 + row;  // the same in both threads
-        const CtSegment &g = *(reinterpret_cast<const CtSegment *>(sm + C::SEG_OFF) + k);
+        CtSegment &g = *(reinterpret_cast<CtSegment *>(sm + C::SEG_OFF) + k);
         if (g.here == 0) continue;
         const bool there = q * 128 + row < g.here;
         const uint32_t mine = q < g.n_q ? g.n : 0, T = g.T, Tq = q ? g.T1 : T;
@@ -1057,6 +1053,16 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
     t5::fence_after();
     if (warp == C::ISSUER) t5::tmem_dealloc(tmem, 512);
     if (tid == 0 && *err_flag) atomicExch(a.c.err, 5u);
+    // Rows whose result is not finite, a warp each.  Not before: one may take as long as all else, and the waits above have a limit.
+    for (uint32_t k = 0, turn = 0; k < pre[CT_PAIRS + 1]; k++) {
+        const CtSegment &g = segs[k];
+        for (uint32_t w = 0; w < CT_ROWS / 32; w++)
+            for (uint32_t rows = g.again[w]; rows; rows &= rows - 1)
+                if (turn++ % (C::THREADS / 32) == warp) {
+                    const uint32_t i = g.r0 + w * 32 + (uint32_t)(__ffs(rows) - 1);
+                    cache_plain_row<KIND, HD>(a, g.x, i / a.group, g.kh * a.group + i % a.group, lane);
+                }
+    }
 }
 
 // ---- host side -----------------------------------------------------------------------------------

@@ -119,3 +119,40 @@ def test_turns_of_rows_over_codes(backend, fmt, rows, hd):
     for sizes in (HALVES, EMPTY, EARLY, TURNS):
         c = Cache(fmt, rows, 1, hd, n_seqs=20, max_len=430, page=32, seed=hd + 3)
         _both(backend, c, sizes, 8, seqs=[i % 20 for i in range(len(sizes))], seed=4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,rows,hd", [("16", "bf16", 64), ("int8", "fp16", 64), ("16", "fp16", 128)])
+def test_many_rows_of_a_long_sequence_taken_again(backend, fmt, rows, hd):
+    """An infinite value early in a sequence of 60000 positions, seen by all of its rows or by some: its row tile is taken
+    again position by position, which takes far longer than the other row tiles of its blocks, and they are right all the same."""
+    sizes = [(32, 300)] * 40 + [(32, 60000)] + [(32, 300)] * 40
+    seqs = [int(i != 40) for i in range(81)]
+    assert blocks_with(sizes, 8, 1, lambda p: p[0] == 40, lambda p: p[0] == 41, whole=False) == 1
+    c = Cache(fmt, rows, 1, hd, n_seqs=2, max_len=60000, page=64, seed=hd + 4)
+    entries, n = _entries(sizes, seqs)
+    q = queries(n, 8, hd, rows, 5)
+    mine = slice(40 * 32, 41 * 32)
+    near = [entries[i] for i in (0, 20, 38, 39, 41, 42, 43, 60, 80)]
+    others = [r0 + i for _, r0, t, _ in near for i in range(t)]
+    want, tol = oracle(c, q, near, 8)
+    page, at = c.place(0, 1000)
+    if fmt == "16":
+        c.pool["v"][page, 0, at, 7] = math.inf
+    else:
+        c.scale["v"][page, 0, at] = math.inf
+    got = run_attention(backend, c, q, entries, 8)
+    check(got, want, tol, others)
+    assert not torch.isfinite(got[mine].float()).all(-1).any()
+    window = 58980  # the last 20 tokens do not see position 1000
+    want, tol = oracle(c, q, near, 8, window=window)
+    got = run_attention(backend, c, q, entries, 8, window=window)
+    check(got, want, tol, others)
+    if fmt == "16":
+        c.pool["v"][page, 0, at, 7] = 0.0
+    else:
+        c.scale["v"][page, 0, at] = 0.0
+    want, tol = oracle(c, q, [entries[40]], 8, window=window)
+    late = [40 * 32 + i for i in range(32) if 59968 + i - window >= 1000]
+    assert 0 < len(late) < 32
+    check(got, want, tol, late)
