@@ -69,53 +69,75 @@ __device__ __forceinline__ bool cache_sees(const CacheAttnDev &a, const CacheEnt
     return c <= r.last && (c > r.low || (uint32_t)c < a.sinks);
 }
 
-// One token's output for one head by one warp in 32 bits, position by position, in three passes: the largest score, the sum of the weights, the
-// values over that sum, which is no larger than the largest of them (values near bf16's largest overflow the sums of the other kernels).  What the formula gives for infinities and NaN is what this gives; positions that the row does not see take no part.
+// One token's output for one head by one warp in 32 bits, in three passes: the largest score, the sum of the weights, the values over that
+// sum, which is no larger than the largest of them (values near bf16's largest overflow the sums of the other kernels).  What the formula
+// gives for infinities and NaN is what this gives; positions that the row does not see take no part.  Scores are a position a lane, the
+// values' sums HD / 32 columns a lane: bound by the latency of the loads, once for 32 positions (60000 positions of a 64-wide head, 256 rows
+// by the 20 warps of a block: 342 ms; a position at a time by the whole warp 1610 ms).
 template <int KIND, int HD>
 __device__ __noinline__ void cache_plain_row(const CacheAttnDev &a, const CacheEntry &x, uint32_t token, uint32_t head, uint32_t lane) {
-    constexpr int VEC = HD / 32;
-    constexpr uint32_t ROWB = HD * kv_bits<KIND>() / 8;
+    constexpr int VEC = HD / 32, PIECE = 128 / (int)kv_bits<KIND>();  // columns of a lane; values of 16 bytes
+    constexpr uint32_t ROWB = HD * kv_bits<KIND>() / 8, ALL = 0xFFFFFFFFu;
     const uint32_t kh = head / a.group, col = lane * VEC;
     const CacheRow r = cache_row(a, x, token);
-    float q[VEC], acc[VEC];
+    const uint16_t *q = a.q + (size_t)(x.row0 + token) * a.q_stride + (size_t)head * HD;
+    float acc[VEC], top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < VEC; i++) {
-        q[i] = kv_row_value(a.q[(size_t)(x.row0 + token) * a.q_stride + (size_t)head * HD + col + i], a.c.rows_bf16);
-        acc[i] = 0.0f;
-    }
-    float top = -INFINITY, sum = 0.0f;
+    for (int i = 0; i < VEC; i++) acc[i] = 0.0f;
     bool any = false;
+    const int32_t gap_lo = (int32_t)min(a.sinks, 0x7FFFFFFFu), gap_hi = min(r.low, x.first - 1);  // what the window leaves out
     for (int pass = 0; pass < 3; pass++) {
-        // positions that no row under this window sees are stepped over
-        const int32_t gap_lo = (int32_t)min(a.sinks, 0x7FFFFFFFu), gap_hi = min(r.low, x.first - 1);
-        for (int32_t p = 0; p < x.len; p++) {
-            if (p >= gap_lo && p <= gap_hi) {
-                p = gap_hi;
+        for (int32_t p0 = 0; p0 < x.len; p0 += 32) {
+            if (p0 >= gap_lo && p0 + 31 <= gap_hi) {       // none of these 32: on to those that gap_hi + 1 is one of
+                p0 = (gap_hi + 1) / 32 * 32 - 32;
                 continue;
             }
-            uint32_t page;
-            if (!cache_sees(a, x, r, p) || !kv_page(a.c, x.seq, (uint32_t)p, page)) continue;
-            const size_t at = kv_row(a.c, page, kh, (uint32_t)p);
-            float k[VEC], v[VEC], d = 0.0f;
-            kv_values<KIND, VEC>(a.c.k + at * ROWB, a.c.ks + at * kv_scales<KIND>(), col, k);
+            const int32_t p = p0 + (int32_t)lane;
+            uint32_t page = 0;
+            const bool see = cache_sees(a, x, r, p) && kv_page(a.c, x.seq, (uint32_t)p, page);
+            unsigned long long at = 0;
+            float d = 0.0f;
+            if (see) {
+                at = kv_row(a.c, page, kh, (uint32_t)p);
+                const uint4 *row = reinterpret_cast<const uint4 *>(a.c.k + at * ROWB);
+#pragma unroll 2
+                for (int c = 0; c < HD / PIECE; c++) {
+                    const uint4 w = __ldg(row + c);
+                    float k[PIECE];
+                    kv_values<KIND, PIECE>(reinterpret_cast<const uint8_t *>(&w), a.c.ks + at * kv_scales<KIND>(), 0, k);
 #pragma unroll
-            for (int i = 0; i < VEC; i++) d = fmaf(q[i], k[i], d);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xFFFFFFFFu, d, o);
-            d *= a.scale;
-            any = true;
+                    for (int i = 0; i < PIECE; i++) d = fmaf(kv_row_value(__ldg(q + c * PIECE + i), a.c.rows_bf16), k[i], d);
+                }
+                d *= a.scale;
+                any = true;
+            }
             if (pass == 0) {
-                top = fmaxf(top, d);
+                if (see) top = fmaxf(top, d);
             } else if (pass == 1) {
-                sum += expf(d - top);
+                if (see) sum += expf(d - top);
             } else {
-                const float w = expf(d - top) / sum;
-                kv_values<KIND, VEC>(a.c.v + at * ROWB, a.c.vs + at * kv_scales<KIND>(), col, v);
+                const float w = see ? expf(d - top) / sum : 0.0f;
+                const uint32_t seen = __ballot_sync(ALL, see);
+#pragma unroll 8
+                for (int u = 0; u < 32; u++) {
+                    const float f = __shfl_sync(ALL, w, u);
+                    const unsigned long long from = __shfl_sync(ALL, at, u);
+                    if (seen >> u & 1) {
+                        float v[VEC];
+                        kv_values<KIND, VEC>(a.c.v + from * ROWB, a.c.vs + from * kv_scales<KIND>(), col, v);
 #pragma unroll
-                for (int i = 0; i < VEC; i++) acc[i] = fmaf(w, v[i], acc[i]);
+                        for (int i = 0; i < VEC; i++) acc[i] = fmaf(f, v[i], acc[i]);
+                    }
+                }
             }
         }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            if (pass == 0) top = fmaxf(top, __shfl_xor_sync(ALL, top, o));
+            if (pass == 1) sum += __shfl_xor_sync(ALL, sum, o);
+        }
     }
+    any = __any_sync(ALL, any);
     uint16_t *dst = a.out + (size_t)(x.row0 + token) * a.out_stride + (size_t)head * HD + col;
 #pragma unroll
     for (int i = 0; i < VEC; i++) dst[i] = kv_round(any ? acc[i] : 0.0f, a.c.rows_bf16);
