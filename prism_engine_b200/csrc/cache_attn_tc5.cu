@@ -10,7 +10,8 @@
 //   codes         three warps load them to registers a tile ahead and store them as fp16 in the swizzle the products read.  Keys stay
 //                 exact codes, their scales multiply the scores; q enters as fp16 over a power of two.  Values are code * scale (+ zero) over
 //                 a power of two of their tile, rounded once: code * (high part) + code * (low part) of the scale in fp16 pairs; a weight is shifted
-//                 by the exponent in which its tile lies below the largest so far.  A value 2^27 below the largest of its tile loses bits.
+//                 by the exponent in which its tile lies below the largest so far.  Where positions' values lie more than 2^16 apart, seen or
+//                 not, the rows are taken by themselves.
 //
 // Positions past the end are zero.  A position that a row does not see meets weight 0, which an infinity there turns into NaN: a row whose
 // result is not finite is taken again by itself (cache_plain_row), after all parts of its block.
@@ -35,6 +36,9 @@ constexpr int CT_SOFT = 16;                                     // softmax warps
 // A row tile costs as many units as it has position tiles, but at least a CT_LEAST-th of the longest: with at most CT_ITEMS row tiles an SM a
 // block has at most CT_ITEMS * CT_LEAST + 2 parts.
 constexpr uint32_t CT_LEAST = 4, CT_ITEMS = 8, CT_SEGMENTS = CT_LEAST * CT_ITEMS + 2;
+// Powers of two that the largest values of two positions of a part may lie apart, seen or not: their rows are taken by themselves else.  With values
+// to 2^14 in fp16, the scale of one 2^16 below is held to 2^-15, and a weight of a tile that far below the others' to 2^-21 of its largest.
+constexpr int CT_APART = 16;
 constexpr float CT_GROW = 3.0f, CT_UP = 12.0f;  // powers of two: what a score may lie above the maximum in use; of the weights in fp16
 // Part of a row tile that a block does.
 struct CtSegment {
@@ -47,12 +51,13 @@ struct CtSegment {
     // barriers go on from part to part: position tiles before this one (T1: with a second tile of rows), parts with such tiles
     uint32_t T, T1, S0, S1;
     uint32_t again[CT_ROWS / 32];         // rows to be taken again by themselves: a bit each
+    uint32_t wide;                        // values of its position tiles lie too far apart for fp16 (CT_APART)
 };
 template <int KIND, int HD>
 struct CtCfg {
     static constexpr int PANELS = HD / 64, PANEL = 128 * 128, TILE = PANELS * PANEL;  // 128 rows of 64 values, in the 128-byte swizzle
     static constexpr int NSC = (int)kv_scales<KIND>(), ROWB = HD * (int)kv_bits<KIND>() / 8;
-    static constexpr int SLOT = NSC ? 2 * CT_POS * NSC * 4 + 16 : 0;                   // key scales, value scales, each converting warp's largest of the latter
+    static constexpr int SLOT = NSC ? 2 * CT_POS * NSC * 4 + 32 : 0;                   // key scales, value scales, each converting warp's largest value by the latter, its smallest but 0
     static constexpr int K_OFF = 2 * TILE, V_OFF = K_OFF + CT_ST * TILE, SC_OFF = V_OFF + CT_ST * TILE, BAR_OFF = SC_OFF + CT_SC * SLOT;
     // barriers: kfull, kempty, vfull, vempty [2 each], sfull, pfull, ofull, qfull [2 each], scales [4]
     static constexpr int STATE_OFF = BAR_OFF + 8 * (4 * CT_ST + 8 + CT_SC);
@@ -159,10 +164,14 @@ __device__ __forceinline__ float ct_max3(float a, uint32_t b, uint32_t c) {
 __device__ __forceinline__ uint32_t ct_below(int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 __device__ __forceinline__ float ct_pow2(int32_t e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
 
-// Exponent of the largest of four numbers, each not negative.
+// Exponent of the largest of four numbers, each not negative; of the smallest.
 __device__ __forceinline__ int32_t ct_exponent(const float *top) {
     const float4 a = *reinterpret_cast<const float4 *>(top);
     return max((int32_t)(__float_as_uint(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w))) >> 23) - 127, -100);
+}
+__device__ __forceinline__ int32_t ct_least_exponent(const float *low) {
+    const float4 a = *reinterpret_cast<const float4 *>(low);
+    return (int32_t)(__float_as_uint(fminf(fminf(a.x, a.y), fminf(a.z, a.w))) >> 23) - 127;
 }
 // Which of 32 positions from c0 on a row sees: the last it sees of the committed, the window's end, the mask.
 __device__ __forceinline__ uint32_t ct_seen(const CacheAttnDev &a, const CacheEntry &x, const CacheRow &r, int32_t c0) {
@@ -302,6 +311,7 @@ __device__ __noinline__ void ct_results(const CtDev &d, CtSegment &g, uint8_t *s
     };
     // ---- results, half of the columns a thread: O times 2^(ref - 13) where V was over a power of two, as the weights' sum is 2^12-fold ----
     const float unit = CODES ? ct_pow2(ref - 13) : 1.0f;
+    if (g.wide) l = __uint_as_float(0x7FC00000u);                  // and so is what this part is joined to
     float inv = 1.0f / l, odd = l > 0.0f && m > -INFINITY ? 0.0f : 1.0f;  // not 0 once an output was not finite; a row without a maximum saw nothing, or only -inf
     const uint32_t rr = g.r0 + q * 128 + row;
     // Half a row a thread, through where its half of q was: the products that read it are complete.
@@ -545,6 +555,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             if (cache_entry(a, pair / d.tiles, x)) t = ct_tiles<true>(a, x, pair % d.tiles);  // the same in all blocks of an item
             if (lane < CT_ROWS / 32) g.again[lane] = 0;
             if (lane == 0) {
+                g.wide = 0;
                 g.x = x;
                 g.r0 = pair % d.tiles * CT_ROWS;
                 g.here = t.here;
@@ -964,9 +975,10 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             }
         };
         for (uint32_t k = 0; k < n_segs; k++) {
-        const CtSegment &g = segs[k];
+        CtSegment &g = segs[k];
         const uint32_t n = g.n, T = g.T;
         const int32_t len = g.x.len;
+        int32_t most_ex = -1000, least_ex = 1000;                  // of all tiles of the part so far
         if (n) {
             page = look(g, 0);
             at_k = units(g, 0, page);
@@ -982,7 +994,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             t5::mbar_wait_warp(b_kempty + 8 * st, ph ^ 1, err_flag);
             // the slot's last readers, the softmax of tile j - 4, came before the products that have just been waited for
             float *ksc = reinterpret_cast<float *>(smem + C::SC_OFF + ((T + j) % CT_SC) * C::SLOT), *vsc = ksc + CT_POS * NSC, *tops = vsc + CT_POS * NSC;
-            float big = 0.0f;
+            float big = 0.0f, small = INFINITY;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const uint32_t row = ct + h * 96;
@@ -993,14 +1005,25 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                 // no value is larger; scales that are not finite count for nothing, their values stay what they are
                 const float most = KIND == KV_INT4 ? fmaf(8.0f, fabsf(scr[1][h].x), fabsf(scr[1][h].y)) : fabsf(scr[1][h].x) * (KIND == KV_INT8 ? 128.0f : 448.0f);
                 if (most < INFINITY) big = fmaxf(big, most);
+                if (most > 0.0f) small = fminf(small, most);
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
-            if (lane == 0) tops[cw] = big;
-            if (ct == 0) tops[3] = 0.0f;                           // ct_exponent reads four
-            t5::mbar_arrive(b_sc + 8 * ((T + j) % CT_SC));
-            asm volatile("bar.sync 9, 96;\n" ::: "memory");        // the largest of all three warps
+            // as whole numbers, which non-negative ones are ordered like
+            big = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(big)));
+            small = __uint_as_float(__reduce_min_sync(0xFFFFFFFFu, __float_as_uint(small)));
+            if (lane == 0) {
+                tops[cw] = big;
+                tops[4 + cw] = small;
+            }
+            if (ct == 0) {                                         // four of each are read
+                tops[3] = 0.0f;
+                tops[7] = INFINITY;
+            }
+            asm volatile("bar.sync 9, 96;\n" ::: "memory");        // those of all three warps
             const float unit = ct_pow2(13 - ct_exponent(tops));
+            most_ex = max(most_ex, ct_exponent(tops));
+            least_ex = min(least_ex, ct_least_exponent(tops + 4));
+            if (ct == 0 && most_ex - least_ex > CT_APART) g.wide = 1;
+            t5::mbar_arrive(b_sc + 8 * ((T + j) % CT_SC));
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const uint32_t row = ct + h * 96;
