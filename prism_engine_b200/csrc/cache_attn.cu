@@ -230,14 +230,16 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
     const uint32_t i_lo = (uint32_t)((uint64_t)n_tiles * split / d.splits), i_hi = (uint32_t)((uint64_t)n_tiles * (split + 1) / d.splits);
     auto pos_of = [&](uint32_t i) { return (int32_t)((i < first_tiles ? i : main_lo + (i - first_tiles)) * TP); };
 
-    // Pages are asked for a tile before its rows, so that no warp waits for the table; pages[u] of 16 positions, the table's own number.
-    uint32_t pages[TP / 16];
+    // Pages are asked for a tile before its rows, so that no warp waits for the table; pages[u] of 16 positions, the table's own number.  Only
+    // where some row of the block sees one of them (bit u of `wanted`): others may be gone.
+    uint32_t pages[TP / 16] = {}, wanted = 0;
     auto look = [&](uint32_t i) {
 #pragma unroll
         for (int u = 0; u < TP / 16; u++) {
             const int32_t p = pos_of(i) + u * 16;
-            pages[u] = 0xFFFFFFFFu;
-            if (i < i_hi && p < x.len) pages[u] = kv_page_number(a.c, x.seq, (uint32_t)p);
+            const bool some = i < i_hi && p < end && (p + 15 >= start || (uint32_t)p < a.sinks);
+            if (some) pages[u] = kv_page_number(a.c, x.seq, (uint32_t)p);
+            wanted = (wanted & ~(1u << u)) | (uint32_t)some << u;
         }
     };
     const uint32_t f_at = cr_at<ROWB>(lane / (ROWB / 16), lane % (ROWB / 16));  // of the lane's first piece
@@ -248,7 +250,7 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
 #pragma unroll
             for (int u = 0; u < TP / 16; u++) {            // a page holds at least 16 positions
                 const int32_t p = p0 + u * 16;
-                const int32_t left = p < x.len && kv_page_ok(a.c, pages[u]) ? x.len - p : 0;
+                const int32_t left = (wanted >> u & 1) && kv_page_ok(a.c, pages[u]) ? x.len - p : 0;
                 const size_t row = left ? kv_row(a.c, pages[u], kh, (uint32_t)p) : 0;
                 const uint8_t *ks = a.c.k + row * ROWB + lane * 16, *vs = a.c.v + row * ROWB + lane * 16;
                 const bool all = left >= 16;

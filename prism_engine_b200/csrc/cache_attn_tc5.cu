@@ -44,7 +44,7 @@ constexpr float CT_GROW = 3.0f, CT_UP = 12.0f;  // powers of two: what a score m
 struct CtSegment {
     CacheEntry x;
     uint32_t item, kh, r0, here, n_q, n;  // row tile of an entry and head, its head, first row, rows, tiles of 128 rows; position tiles of this part
-    int32_t i_lo, first, main;            // the first of them; CtTiles
+    int32_t i_lo, first, main, start, end;  // the first of them; CtTiles
     uint32_t whole;                       // the whole row tile
     uint32_t units, from, take;           // of the row tile, of this part
     uint32_t b0, b1, slot, slot0;         // blocks that have parts of the item; places of this block's part and of b0's
@@ -86,12 +86,13 @@ namespace {
 struct CtTiles {
     uint32_t here;              // rows of the tile
     int32_t first, main, all;   // `all` of them
+    int32_t start, end;         // seen by some row: positions below end that are not below start, and the first a.sinks
 };
 // WARP: called by whole warps, which share the rows of a tree.
 template <bool WARP>
 __device__ __forceinline__ CtTiles ct_tiles(const CacheAttnDev &a, const CacheEntry &x, uint32_t tile) {
     const uint32_t n_rows = x.n * a.group, r0 = tile * CT_ROWS;
-    CtTiles t{r0 < n_rows ? min((uint32_t)CT_ROWS, n_rows - r0) : 0, 0, 0, 0};
+    CtTiles t{r0 < n_rows ? min((uint32_t)CT_ROWS, n_rows - r0) : 0, 0, 0, 0, 0, 0};
     if (t.here == 0) return t;
     const uint32_t tok_lo = r0 / a.group, tok_hi = (r0 + t.here - 1) / a.group;
     int32_t low = -1;
@@ -106,6 +107,8 @@ __device__ __forceinline__ CtTiles ct_tiles(const CacheAttnDev &a, const CacheEn
     t.first = end > 0 ? (int32_t)(min((uint32_t)end, a.sinks) + CT_POS - 1) / CT_POS : 0;
     t.main = max(start / CT_POS, t.first);
     t.all = t.first + max(main_hi - t.main, 0);
+    t.start = start;
+    t.end = end;
     return t;
 }
 
@@ -562,6 +565,8 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                 g.n_q = (t.here + 127) / 128;
                 g.first = t.first;
                 g.main = t.main;
+                g.start = t.start;
+                g.end = t.end;
                 g.i_lo = (int32_t)((int64_t)t.all * g.from / g.units);
                 g.n = (uint32_t)((int32_t)((int64_t)t.all * (g.from + g.take) / g.units) - g.i_lo);
             }
@@ -589,6 +594,9 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         const int32_t i = g.i_lo + (int32_t)j;
         return (i < g.first ? i : g.main + (i - g.first)) * CT_POS;
     };
+
+    // Whether some row of the part sees one of `span` positions from p on: pages of others are not asked for, they may be gone.
+    auto wanted = [&](const CtSegment &g, int32_t p, int32_t span) { return p < g.end && (p + span > g.start || (uint32_t)p < a.sinks); };
 
     if (warp < CT_SOFT) {
         // ================= softmax: two threads a query row, positions 0..63 and 64..127 of a tile =================
@@ -877,8 +885,8 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         if (warp == CT_SOFT) {
             const uint32_t boxes = CT_POS / d.box, b = lane % boxes;
             auto look = [&](const CtSegment &g, uint32_t j) {
-                const int32_t p = j < g.n ? pos_of(g, j) + (int32_t)(b * d.box) : g.x.len;
-                return p < g.x.len ? kv_page_number(a.c, g.x.seq, (uint32_t)p) : 0xFFFFFFFFu;
+                const int32_t p = j < g.n ? pos_of(g, j) + (int32_t)(b * d.box) : 0;
+                return j < g.n && wanted(g, p, (int32_t)d.box) ? kv_page_number(a.c, g.x.seq, (uint32_t)p) : 0xFFFFFFFFu;
             };
             auto load = [&](const CUtensorMap *map, uint32_t dst, uint32_t at, uint32_t mbar) {
                 if (lane == 0) t5::mbar_arrive_expect_tx(mbar, CT_POS * HD * 2);
@@ -894,7 +902,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                     const uint32_t st = (g.T + j) % ST, ph = ((g.T + j) / ST) & 1;
                     const int32_t p = pos_of(g, j) + (int32_t)(b * d.box);
                     // past the last row of the pool: zeros
-                    const uint32_t at = p < g.x.len && kv_page_ok(a.c, page) ? (uint32_t)kv_row(a.c, page, g.kh, (uint32_t)p) : d.pool_rows;
+                    const uint32_t at = wanted(g, p, (int32_t)d.box) && kv_page_ok(a.c, page) ? (uint32_t)kv_row(a.c, page, g.kh, (uint32_t)p) : d.pool_rows;
                     page = look(g, j + 1);
                     t5::mbar_wait_warp(b_kempty + 8 * st, ph ^ 1, err_flag);
                     load(&kmap, base + C::K_OFF + st * C::TILE, at, b_kfull + 8 * st);
@@ -930,12 +938,12 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         uint32_t at_k = 0, at_v = 0;                               // lanes 0..7: the pool row of the tile's 16-position unit (0 where there is none)
         // Pages are asked for two tiles ahead, so that nothing waits for the table.
         auto look = [&](const CtSegment &g, uint32_t j) {
-            const int32_t p = j < g.n ? pos_of(g, j) + (int32_t)(lane & 7) * 16 : g.x.len;
-            return p < g.x.len ? kv_page_number(a.c, g.x.seq, (uint32_t)p) : 0xFFFFFFFFu;
+            const int32_t p = j < g.n ? pos_of(g, j) + (int32_t)(lane & 7) * 16 : 0;
+            return j < g.n && wanted(g, p, 16) ? kv_page_number(a.c, g.x.seq, (uint32_t)p) : 0xFFFFFFFFu;
         };
         auto units = [&](const CtSegment &g, uint32_t j, uint32_t page) {
-            const int32_t p = j < g.n ? pos_of(g, j) + (int32_t)(lane & 7) * 16 : g.x.len;
-            return p < g.x.len && kv_page_ok(a.c, page) ? (uint32_t)kv_row(a.c, page, g.kh, (uint32_t)p) : 0u;
+            const int32_t p = j < g.n ? pos_of(g, j) + (int32_t)(lane & 7) * 16 : 0;
+            return j < g.n && wanted(g, p, 16) && kv_page_ok(a.c, page) ? (uint32_t)kv_row(a.c, page, g.kh, (uint32_t)p) : 0u;
         };
         uint32_t page;
         // Four pieces at a time, so that what they wait for overlaps.
@@ -948,21 +956,23 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             for (int i = 0; i < G; i++)
                 if (first + i < MINE) reg[first + i] = t5::ldg128_nc(pool + (size_t)(at[i] + ((row0 + (first + i) * STEP) & 15)) * C::ROWB + piece * 16);
         };
-        // Past the end some row of the pool is read; its scale is 0, but a code of e4m3 may be NaN.
-        auto clear = [&](int32_t p0, int32_t len) {
-            if (KIND == KV_E4M3 && p0 + CT_POS > len) {
+        // Where no row looks some row of the pool is read; its scale is 0, but a code of e4m3 may be NaN.
+        auto clear = [&](const CtSegment &g, int32_t p0) {
+            if (KIND == KV_E4M3 && (p0 + CT_POS > g.end || p0 < g.start)) {
 #pragma unroll
-                for (int i = 0; i < MINE; i++)
-                    if (p0 + (int32_t)(row0 + i * STEP) >= len) reg[i] = make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < MINE; i++) {
+                    const int32_t row = (int32_t)(row0 + i * STEP);
+                    if (p0 + row >= g.x.len || !wanted(g, p0 + (row & ~15), 16)) reg[i] = make_uint4(0, 0, 0, 0);
+                }
             }
         };
         constexpr int FULL = CT_POS / STEP;                        // pieces that every thread has
-        auto load_scales = [&](int32_t p0, int32_t len, uint32_t of) {
+        auto load_scales = [&](const CtSegment &g, int32_t p0, uint32_t of) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const uint32_t row = ct + h * 96, at = __shfl_sync(0xFFFFFFFFu, of, (row >> 4) & 7);
                 scr[0][h] = scr[1][h] = make_float2(0.0f, 0.0f);
-                if (row < CT_POS && p0 + (int32_t)row < len) {
+                if (row < CT_POS && p0 + (int32_t)row < g.x.len && wanted(g, p0 + (int32_t)(row & ~15u), 16)) {
                     const size_t from = ((size_t)at + (row & 15)) * NSC;
                     if constexpr (NSC == 2) {
                         scr[0][h] = __ldg(reinterpret_cast<const float2 *>(a.c.ks + from));
@@ -977,7 +987,6 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         for (uint32_t k = 0; k < n_segs; k++) {
         CtSegment &g = segs[k];
         const uint32_t n = g.n, T = g.T;
-        const int32_t len = g.x.len;
         int32_t most_ex = -1000, least_ex = 1000;                  // of all tiles of the part so far
         if (n) {
             page = look(g, 0);
@@ -985,11 +994,11 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             page = look(g, 1);
 #pragma unroll
             for (int i = 0; i < MINE; i += G) load(a.c.k, i, at_k);
-            load_scales(pos_of(g, 0), len, at_k);
+            load_scales(g, pos_of(g, 0), at_k);
         }
         for (uint32_t j = 0; j < n; j++) {
             const uint32_t st = (T + j) % ST, ph = ((T + j) / ST) & 1;
-            const int32_t now = pos_of(g, j), next = j + 1 < n ? pos_of(g, j + 1) : len;  // nothing is loaded from the end on
+            const int32_t now = pos_of(g, j), next = j + 1 < n ? pos_of(g, j + 1) : g.x.len;  // nothing is loaded from the end on
             at_v = at_k;
             t5::mbar_wait_warp(b_kempty + 8 * st, ph ^ 1, err_flag);
             // the slot's last readers, the softmax of tile j - 4, came before the products that have just been waited for
@@ -1035,9 +1044,9 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             }
             at_k = units(g, j + 1, page);
             page = look(g, j + 2);
-            load_scales(next, len, at_k);
+            load_scales(g, next, at_k);
             const uint32_t kt = base + C::K_OFF + st * C::TILE, vt = base + C::V_OFF + st * C::TILE;
-            clear(now, len);
+            clear(g, now);
 #pragma unroll
             for (int f = 0; f < MINE; f += G) {
 #pragma unroll
@@ -1050,7 +1059,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             asm volatile("bar.sync 9, 96;\n" ::: "memory");        // the scales of all three warps
             t5::mbar_wait_warp(b_vempty + 8 * st, ph ^ 1, err_flag);
             const uint32_t v_at = base + C::SC_OFF + ((T + j) % CT_SC) * C::SLOT + (CT_POS + row0) * NSC * 4;
-            clear(now, len);
+            clear(g, now);
 #pragma unroll
             for (int f = 0; f < MINE; f += G) {
                 float2 sc[G];

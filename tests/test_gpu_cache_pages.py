@@ -1,0 +1,54 @@
+"""Tables whose pages are not all there: pages that no row sees are not asked for, whatever the kernel.  Bound per output as in
+test_gpu_cache_many_rows."""
+import pytest
+import torch
+
+from cache_util import Cache, check, queries, run_attention
+from test_gpu_cache_many_rows import _entries, oracle
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = [("16", "fp16"), ("16", "bf16"), ("int8", "fp16"), ("e4m3", "bf16"), ("int4", "bf16")]
+
+
+def _seen(entries, n_seqs, most, window, sinks, q_pos=None):
+    """[sequence, position]: whether some row sees it (drafted positions: all)."""
+    see = torch.zeros(n_seqs, most, dtype=torch.bool)
+    for s, r0, n, length in entries:
+        for i in range(n):
+            p = q_pos[r0 + i] if q_pos else length - n + i
+            c = torch.arange(most)
+            see[s] |= (c < length - n if q_pos else c <= p) & ((c > p - window) | (c < sinks))
+        if q_pos:
+            see[s, length - n:length] = True
+    return see
+
+
+def _give_back(c, see):
+    """Table entries of pages with nothing to see are no pages."""
+    gone = ~see.view(c.n_seqs, -1, c.page).any(-1)
+    assert gone.any() and not gone.all()
+    odd = torch.tensor([-1, c.pages, 1 << 30], dtype=torch.int32)
+    c.table.copy_(torch.where(gone, odd[torch.arange(gone.numel()) % 3].view_as(gone), c.table_cpu).cuda())
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (37, 5), (100, 16), (300, 70)])
+@pytest.mark.parametrize("page", [16, 32, 128, 256])
+@pytest.mark.parametrize("fmt,rows", FORMATS)
+def test_pages_behind_the_window_given_back(backend, fmt, rows, page, window, sinks):
+    """Single tokens, small portions and large ones; tokens and drafts."""
+    for hd, heads, kvh, sizes in ((64, 6, 2, [(1, 500), (1, 511), (2, 512), (1, 3)]), (256, 4, 1, [(3, 700)]), (32, 4, 1, [(5, 333), (1, 1024)]),
+                                  (128, 8, 1, [(40, 600 + 13 * i) for i in range(24)]), (64, 16, 1, [(17 + i, 900 - 31 * i) for i in range(20)]),
+                                  (128, 16, 1, [(70, 1000)])):
+        most = -(-1024 // page) * page
+        c = Cache(fmt, rows, kvh, hd, n_seqs=len(sizes), max_len=most, page=page, seed=hd)
+        entries, n = _entries(sizes, list(range(len(sizes))))
+        q = queries(n, heads, hd, rows, 1)
+        _give_back(c, _seen(entries, len(sizes), most, window, sinks))
+        want, tol = oracle(c, q, entries, heads, window=window, sinks=sinks)
+        check(run_attention(backend, c, q, entries, heads, window=window, sinks=sinks), want, tol)
+        pos = [length - t + i % 3 for t, length in sizes for i in range(t)]
+        masks = [(1 << i % 64) | 1 for t, _ in sizes for i in range(t)]
+        _give_back(c, _seen(entries, len(sizes), most, window, sinks, pos))
+        want, tol = oracle(c, q, entries, heads, window=window, sinks=sinks, masks=masks, q_pos=pos)
+        check(run_attention(backend, c, q, entries, heads, window=window, sinks=sinks, masks=masks, q_pos=pos), want, tol)
