@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
         }
     };
     const uint32_t f_at = cr_at<ROWB>(lane / (ROWB / 16), lane % (ROWB / 16));  // of the lane's first piece
+    uint32_t skip = 0;                                     // two bits a stage: 16 positions whose page is none, nobody's from here on
     auto fetch = [&](uint32_t i, uint32_t st) {
         if (i < i_hi) {
             const uint32_t kt = ring + st * C::STAGE, vt = kt + C::TILE, ksc = vt + C::TILE, vsc = ksc + C::SCB;
@@ -250,7 +251,11 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
 #pragma unroll
             for (int u = 0; u < TP / 16; u++) {            // a page holds at least 16 positions
                 const int32_t p = p0 + u * 16;
-                const int32_t left = (wanted >> u & 1) && kv_page_ok(a.c, pages[u]) ? x.len - p : 0;
+                int32_t left = wanted >> u & 1 ? x.len - p : 0;
+                if (left && !kv_page_ok(a.c, pages[u])) {
+                    left = 0;
+                    skip |= 1u << (st * 2 + u);
+                }
                 const size_t row = left ? kv_row(a.c, pages[u], kh, (uint32_t)p) : 0;
                 const uint8_t *ks = a.c.k + row * ROWB + lane * 16, *vs = a.c.v + row * ROWB + lane * 16;
                 const bool all = left >= 16;
@@ -483,7 +488,9 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
                 }
         }
         const bool whole = p0 + TP - 1 <= all_to && (p0 > low_max || (uint32_t)(p0 + TP) <= a.sinks);
-        if (!whole) {
+        const uint32_t gone = skip >> (st * 2) & 3;
+        if (!whole || gone) {
+            skip &= ~(3u << (st * 2));
 #pragma unroll
             for (int n = 0; n < NQ; n++)
 #pragma unroll
@@ -499,7 +506,7 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
                                 see = r.mask && p < x.len;
                                 if (see) see = __ldg(r.mask + ((uint32_t)(p - x.first) >> 6)) >> ((p - x.first) & 63) & 1;
                             }
-                            if (!see) s[j][n][2 * c + h] = -INFINITY;
+                            if (!see || (gone >> j & 1)) s[j][n][2 * c + h] = -INFINITY;
                         }
                 }
         }

@@ -888,10 +888,19 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                 const int32_t p = j < g.n ? pos_of(g, j) + (int32_t)(b * d.box) : 0;
                 return j < g.n && wanted(g, p, (int32_t)d.box) ? kv_page_number(a.c, g.x.seq, (uint32_t)p) : 0xFFFFFFFFu;
             };
-            auto load = [&](const CUtensorMap *map, uint32_t dst, uint32_t at, uint32_t mbar) {
-                if (lane == 0) t5::mbar_arrive_expect_tx(mbar, CT_POS * HD * 2);
+            // `none`: boxes of a page that is none; keys there are NaN, so that the rows that look at them are taken again, which skips them
+            auto load = [&](const CUtensorMap *map, uint32_t dst, uint32_t at, uint32_t mbar, uint32_t none) {
+                for (uint32_t m = none; m; m &= m - 1)
+                    for (uint32_t u = lane; u < d.box * 8 * C::PANELS; u += 32)
+                        ct_sts(dst + u / (d.box * 8) * C::PANEL + (uint32_t)(__ffs(m) - 1) * d.box * 128 + u % (d.box * 8) * 16,
+                               make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu));
+                if (none) {
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    __syncwarp();
+                }
+                if (lane == 0) t5::mbar_arrive_expect_tx(mbar, (boxes - __popc(none)) * d.box * HD * 2);
                 __syncwarp();
-                if (lane < boxes)
+                if (lane < boxes && !(none >> lane & 1))
                     for (uint32_t q = 0; q < (uint32_t)C::PANELS; q++)
                         t5::tma_2d(dst + q * C::PANEL + b * d.box * 128, map, (int32_t)(q * 64), (int32_t)at, mbar);
             };
@@ -902,12 +911,13 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
                     const uint32_t st = (g.T + j) % ST, ph = ((g.T + j) / ST) & 1;
                     const int32_t p = pos_of(g, j) + (int32_t)(b * d.box);
                     // past the last row of the pool: zeros
-                    const uint32_t at = wanted(g, p, (int32_t)d.box) && kv_page_ok(a.c, page) ? (uint32_t)kv_row(a.c, page, g.kh, (uint32_t)p) : d.pool_rows;
+                    const bool some = wanted(g, p, (int32_t)d.box), there = some && kv_page_ok(a.c, page);
+                    const uint32_t at = there ? (uint32_t)kv_row(a.c, page, g.kh, (uint32_t)p) : d.pool_rows, none = __ballot_sync(0xFFFFFFFFu, some && !there && lane < boxes);
                     page = look(g, j + 1);
                     t5::mbar_wait_warp(b_kempty + 8 * st, ph ^ 1, err_flag);
-                    load(&kmap, base + C::K_OFF + st * C::TILE, at, b_kfull + 8 * st);
+                    load(&kmap, base + C::K_OFF + st * C::TILE, at, b_kfull + 8 * st, none);
                     t5::mbar_wait_warp(b_vempty + 8 * st, ph ^ 1, err_flag);
-                    load(&vmap, base + C::V_OFF + st * C::TILE, at, b_vfull + 8 * st);
+                    load(&vmap, base + C::V_OFF + st * C::TILE, at, b_vfull + 8 * st, 0);
                 }
             }
             // every copy in flight lands before the CTA leaves
@@ -935,7 +945,10 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         }
         uint4 reg[MINE];
         float2 scr[2][2];                                          // keys', values' scales of positions ct and ct + 96
-        uint32_t at_k = 0, at_v = 0;                               // lanes 0..7: the pool row of the tile's 16-position unit (0 where there is none)
+        // lanes 0..7: the pool row of the tile's 16-position unit; NO_PAGE where there is none: the scales of its keys are NaN, so that the rows
+        // that look at them are taken again, which skips them
+        uint32_t at_k = 0, at_v = 0;
+        constexpr uint32_t NO_PAGE = 0x80000000u;
         // Pages are asked for two tiles ahead, so that nothing waits for the table.
         auto look = [&](const CtSegment &g, uint32_t j) {
             const int32_t p = j < g.n ? pos_of(g, j) + (int32_t)(lane & 7) * 16 : 0;
@@ -943,7 +956,8 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         };
         auto units = [&](const CtSegment &g, uint32_t j, uint32_t page) {
             const int32_t p = j < g.n ? pos_of(g, j) + (int32_t)(lane & 7) * 16 : 0;
-            return j < g.n && wanted(g, p, 16) && kv_page_ok(a.c, page) ? (uint32_t)kv_row(a.c, page, g.kh, (uint32_t)p) : 0u;
+            if (j >= g.n || !wanted(g, p, 16)) return 0u;
+            return kv_page_ok(a.c, page) ? (uint32_t)kv_row(a.c, page, g.kh, (uint32_t)p) : NO_PAGE;
         };
         uint32_t page;
         // Four pieces at a time, so that what they wait for overlaps.
@@ -951,7 +965,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         auto load = [&](const uint8_t *pool, int first, uint32_t of) {
             uint32_t at[G];
 #pragma unroll
-            for (int i = 0; i < G; i++) at[i] = __shfl_sync(0xFFFFFFFFu, of, ((row0 + (first + i) * STEP) >> 4) & 7);
+            for (int i = 0; i < G; i++) at[i] = __shfl_sync(0xFFFFFFFFu, of, ((row0 + (first + i) * STEP) >> 4) & 7) & ~NO_PAGE;
 #pragma unroll
             for (int i = 0; i < G; i++)
                 if (first + i < MINE) reg[first + i] = t5::ldg128_nc(pool + (size_t)(at[i] + ((row0 + (first + i) * STEP) & 15)) * C::ROWB + piece * 16);
@@ -972,7 +986,9 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             for (int h = 0; h < 2; h++) {
                 const uint32_t row = ct + h * 96, at = __shfl_sync(0xFFFFFFFFu, of, (row >> 4) & 7);
                 scr[0][h] = scr[1][h] = make_float2(0.0f, 0.0f);
-                if (row < CT_POS && p0 + (int32_t)row < g.x.len && wanted(g, p0 + (int32_t)(row & ~15u), 16)) {
+                if (at & NO_PAGE) {
+                    scr[0][h].x = __uint_as_float(0x7FC00000u);
+                } else if (row < CT_POS && p0 + (int32_t)row < g.x.len && wanted(g, p0 + (int32_t)(row & ~15u), 16)) {
                     const size_t from = ((size_t)at + (row & 15)) * NSC;
                     if constexpr (NSC == 2) {
                         scr[0][h] = __ldg(reinterpret_cast<const float2 *>(a.c.ks + from));
