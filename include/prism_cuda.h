@@ -357,8 +357,9 @@ typedef struct prism_cache_attention {
     uint32_t tree_words;     /* at least (max_tokens + 63) / 64 */
     const int32_t *q_pos;    /* [n_rows], device; read with a tree under a window */
 } prism_cache_attention;
-/* Captured calls use memory of their capture, which the context keeps; calls of one context, and replays of one capture, do not
- * overlap. */
+/* Captured calls use memory of their capture (tens of MB where blocks share work).  Later captures of the context take it when the graph
+ * and all that was instantiated from it are destroyed; it is given back with the context, or when an eager call needs more than
+ * it has.  Calls of one context, and replays of one capture, do not overlap. */
 int prism_cuda_cache_attention_dev(prism_cuda_ctx *ctx, const prism_cache *cache, const prism_cache_attention *a);
 
 /* argmax (engine_impl.rs:1448-1459): first strictly greatest. */

@@ -23,7 +23,9 @@
 // 64 heads of 128 over 8, a token of 32 sequences under a window of 4096: 16 bits 85 us (6.3 TB/s), int8 63 us (4.4 TB/s), int4 64 us; one sequence of 131071
 // positions: 16 bits 93 us (5.8 TB/s), int4 56 us (2.7 TB/s); 14 heads of 64 over 2, 516 visible positions: 5.5 us.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <memory>
 #include <stdexcept>
 #include <vector>
 
@@ -766,12 +768,15 @@ __global__ void __launch_bounds__(CR_THREADS, CrCfg<KIND, HD, NQ>::BLOCKS) cache
 
 // ---- scratch -----------------------------------------------------------------------------------------------------------------
 // Parts and counters.  Eager calls of a context share a block, which grows when the stream is idle.  Calls that are being captured use
-// a block of their capture, kept until the context goes: a replay finds it whatever ran in between, and no two captures share one.
+// a block of their capture: a replay finds it whatever ran in between, and no two captures share one.  The captured graph and what is
+// instantiated from it hold a reference to the block; when the last of them is gone, and its launches with it, a later capture takes it.
 struct CacheScratch {
     struct Block {
         unsigned long long capture;  // 0: eager
         uint8_t *mem;
         size_t part_bytes, counts;
+        std::shared_ptr<std::atomic<bool>> left;  // of a capture: nothing refers to it any more
+        bool fits(size_t bytes, size_t n) const { return part_bytes >= bytes && counts >= n; }
     };
     std::vector<Block> blocks;
 };
@@ -780,37 +785,79 @@ void cache_scratch_free(CacheScratch *s) {
     for (auto &b : s->blocks) cudaFree(b.mem);
     delete s;
 }
+static void CUDART_CB cache_block_left(void *p) {          // on a thread of the driver's: no CUDA calls
+    auto *left = static_cast<std::shared_ptr<std::atomic<bool>> *>(p);
+    (*left)->store(true);
+    delete left;
+}
+// The block goes with this graph.
+static int cache_block_of(prism_cuda_ctx *ctx, CacheScratch::Block &b, unsigned long long capture, cudaGraph_t graph) {
+    auto flag = std::make_shared<std::atomic<bool>>(false);
+    auto theirs = std::make_unique<std::shared_ptr<std::atomic<bool>>>(flag);
+    cudaUserObject_t object;
+    PRISM_CUDA_TRY(ctx, cudaUserObjectCreate(&object, theirs.get(), cache_block_left, 1, cudaUserObjectNoDestructorSync));
+    theirs.release();
+    b.capture = capture;
+    b.left = std::move(flag);
+    const cudaError_t e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+    if (e != cudaSuccess) {
+        (void)cudaUserObjectRelease(object, 1);
+        return cuda_fail(ctx, e, "cudaGraphRetainUserObject");
+    }
+    return PRISM_OK;
+}
 int cache_scratch(prism_cuda_ctx *ctx, size_t part_bytes, size_t counts, float **part, unsigned int **count) {
     if (!ctx->cache_scratch) ctx->cache_scratch = new CacheScratch();
     auto &blocks = ctx->cache_scratch->blocks;
     cudaStreamCaptureStatus status;
     unsigned long long id = 0;
-    PRISM_CUDA_TRY(ctx, cudaStreamGetCaptureInfo(ctx->stream, &status, &id));
+    cudaGraph_t graph = nullptr;
+    PRISM_CUDA_TRY(ctx, cudaStreamGetCaptureInfo(ctx->stream, &status, &id, &graph));
     if (status == cudaStreamCaptureStatusNone) id = 0;
-    for (size_t i = 0; i < blocks.size(); i++) {
-        auto &b = blocks[i];
-        if (b.capture != id) continue;
-        if (b.part_bytes >= part_bytes && b.counts >= counts) {
-            *part = reinterpret_cast<float *>(b.mem);
-            if (count) *count = reinterpret_cast<unsigned int *>(b.mem + b.part_bytes);
+    auto use = [&](CacheScratch::Block &b) {
+        *part = reinterpret_cast<float *>(b.mem);
+        if (count) *count = reinterpret_cast<unsigned int *>(b.mem + b.part_bytes);
+    };
+    // kernels leave the counters at zero; in a capture this is a node before them
+    auto clear = [&](CacheScratch::Block &b) -> int {
+        if (b.counts) PRISM_CUDA_TRY(ctx, cudaMemsetAsync(b.mem + b.part_bytes, 0, b.counts * 4, ctx->stream));
+        return PRISM_OK;
+    };
+    for (auto &b : blocks)
+        if (b.capture == id && b.fits(part_bytes, counts)) {
+            use(b);
             return PRISM_OK;
         }
-        if (id == 0) {
-            PRISM_CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream));
-            part_bytes = std::max(part_bytes, b.part_bytes);
-            counts = std::max(counts, b.counts);
-            cudaFree(b.mem);
+    if (id == 0) {                                         // the block in use, and those that nothing refers to, make room for a larger one
+        PRISM_CUDA_TRY(ctx, cudaStreamSynchronize(ctx->stream));
+        for (size_t i = blocks.size(); i-- > 0;) {
+            if (blocks[i].capture != 0 && !blocks[i].left->load()) continue;
+            if (blocks[i].capture == 0) {
+                part_bytes = std::max(part_bytes, blocks[i].part_bytes);
+                counts = std::max(counts, blocks[i].counts);
+            }
+            cudaFree(blocks[i].mem);
             blocks.erase(blocks.begin() + i);
-            break;
+        }
+    } else {
+        CacheScratch::Block *best = nullptr;
+        for (auto &b : blocks)
+            if (b.capture != 0 && b.left->load() && b.fits(part_bytes, counts) && (!best || b.part_bytes < best->part_bytes)) best = &b;
+        if (best) {
+            PRISM_TRY(cache_block_of(ctx, *best, id, graph));
+            PRISM_TRY(clear(*best));
+            use(*best);
+            return PRISM_OK;
         }
     }
     blocks.reserve(blocks.size() + 1);                     // nothing throws between the allocation and its place
     part_bytes = (part_bytes + 255) / 256 * 256;
     counts = (counts + 63) / 64 * 64;
-    CacheScratch::Block b{id, nullptr, part_bytes, counts};
+    CacheScratch::Block b{id, nullptr, part_bytes, counts, nullptr};
     if (id == 0) {
         PRISM_CUDA_TRY(ctx, device_malloc(ctx, (void **)&b.mem, part_bytes + counts * 4));
     } else {
+        b.left = std::make_shared<std::atomic<bool>>(true);  // until the graph has it
         cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // an allocation is no part of the capture
         PRISM_CUDA_TRY(ctx, cudaThreadExchangeStreamCaptureMode(&mode));
         const cudaError_t e = cudaMalloc((void **)&b.mem, part_bytes + counts * 4);
@@ -820,11 +867,10 @@ int cache_scratch(prism_cuda_ctx *ctx, size_t part_bytes, size_t counts, float *
             return cuda_fail(ctx, e, "cudaMalloc(attention scratch of a capture)");
         }
     }
-    blocks.push_back(b);
-    // kernels leave the counters at zero; in a capture this is a node before them
-    if (counts) PRISM_CUDA_TRY(ctx, cudaMemsetAsync(b.mem + part_bytes, 0, counts * 4, ctx->stream));
-    *part = reinterpret_cast<float *>(b.mem);
-    if (count) *count = reinterpret_cast<unsigned int *>(b.mem + part_bytes);
+    blocks.push_back(std::move(b));
+    if (id != 0) PRISM_TRY(cache_block_of(ctx, blocks.back(), id, graph));
+    PRISM_TRY(clear(blocks.back()));
+    use(blocks.back());
     return PRISM_OK;
 }
 
