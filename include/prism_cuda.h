@@ -298,7 +298,7 @@ int prism_cuda_attention_step_kv(prism_cuda_ctx *ctx, uint32_t layer, const uint
  *                       zero = lo + 8 * scale; element 2i in the low half of byte i
  * amax, lo, hi: over one head of one position; every step one rounded 32-bit operation.  A span below 2^-100 gives scale 0; a
  * head with a value that is not finite reads back as NaN throughout.
- * Pages, scales and rows are 16-byte aligned device memory.  The calls run on the context's stream and return; places are in
+ * Pages, scales and rows are 16-byte aligned device memory, arrays of 32-bit numbers 4-byte aligned.  The calls run on the context's stream and return; places are in
  * device arrays, so a captured call can be replayed with others.  A place outside the cache, or whose page is not one of the
  * pool's, is skipped, and the next synchronising call returns PRISM_E_ARG; a negative sequence or position is padding and
  * skipped without that. */

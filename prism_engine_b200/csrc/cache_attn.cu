@@ -965,6 +965,8 @@ static int cache_attention(prism_cuda_ctx *ctx, const prism_cache *c, const pris
     if (p->q_stride < width || p->out_stride < width || p->q_stride % 8 || p->out_stride % 8 ||
         ((reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->out)) & 15))
         return fail(ctx, PRISM_E_ARG, "cache_attention: rows must be 16-byte aligned and at least num_heads * head_dim values apart");
+    if (!kv_words(p->seq, p->q_start, p->length, p->q_pos))
+        return fail(ctx, PRISM_E_ARG, "cache_attention: seq, q_start, length and q_pos must be 4-byte aligned");
     if (reinterpret_cast<uintptr_t>(p->tree) & 7) return fail(ctx, PRISM_E_ARG, "cache_attention: masks must be 8-byte aligned");
     if (p->q == p->out) return fail(ctx, PRISM_E_ARG, "cache_attention: results must not overlap the queries");  // a row may be taken again
     DeviceGuard on(ctx->device);

@@ -389,6 +389,7 @@ static int cache_rows(prism_cuda_ctx *ctx, const prism_cache *c, bool write, con
     const uint64_t width = (uint64_t)c->kv_heads * c->head_dim;
     if (k_stride < width || v_stride < width || k_stride % 8 || v_stride % 8 || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15))
         return fail(ctx, PRISM_E_ARG, std::string(name) + ": rows must be 16-byte aligned and at least kv_heads * head_dim values apart");
+    if (!kv_words(seq, pos)) return fail(ctx, PRISM_E_ARG, std::string(name) + ": places must be 4-byte aligned");
     if ((uint64_t)n_rows * 2 * c->kv_heads > 0x7FFFFFFFull) return fail(ctx, PRISM_E_ARG, std::string(name) + ": too many rows in one call");
     DeviceGuard on(ctx->device);
     if (on.err != cudaSuccess) return cuda_fail(ctx, on.err, "cudaSetDevice");
@@ -418,6 +419,7 @@ static int cache_keep(prism_cuda_ctx *ctx, const prism_cache *c, uint32_t n_entr
     PRISM_TRY(kv_check(ctx, c, &a.c, &kind));
     if (n_entries == 0 || path_stride == 0) return PRISM_OK;
     if (!seq || !base || !path || !kept) return fail(ctx, PRISM_E_NULL, "cache_keep: null argument");
+    if (!kv_words(seq, base, path, kept)) return fail(ctx, PRISM_E_ARG, "cache_keep: seq, base, path and kept must be 4-byte aligned");
     if (n_entries > 65535) return fail(ctx, PRISM_E_ARG, "cache_keep: at most 65535 entries a call");
     if (path_stride > 0x7FFFFFFFu) return fail(ctx, PRISM_E_ARG, "cache_keep: path_stride is counted in 31 bits");
     DeviceGuard on(ctx->device);

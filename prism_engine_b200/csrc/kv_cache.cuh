@@ -93,6 +93,10 @@ __device__ __forceinline__ void kv_values(const uint8_t *row, const float *sc, u
 }
 #endif
 
+// Whether arrays of 32-bit numbers lie on 4-byte boundaries; others would fault the kernels that read them.
+template <typename... P>
+inline bool kv_words(const P *...p) { return ((reinterpret_cast<uintptr_t>(p) | ...) & 3) == 0; }
+
 // The library's own record of a prism_cache, after its checks.
 int kv_check(prism_cuda_ctx *ctx, const prism_cache *c, KvDev *out, int *kind);
 
