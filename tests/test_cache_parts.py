@@ -156,3 +156,19 @@ def test_many_rows_of_a_long_sequence_taken_again(backend, fmt, rows, hd):
     late = [40 * 32 + i for i in range(32) if 59968 + i - window >= 1000]
     assert 0 < len(late) < 32
     check(got, want, tol, late)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("fmt,rows,hd", CODED)
+def test_ragged_drafts_over_codes(backend, fmt, rows, hd, seed):
+    """Drafts of 2 to 63 tokens behind 200 to 3000 committed ones, and single tokens, neighbouring sequences' values 2^6-fold apart."""
+    g = torch.Generator().manual_seed(seed)
+    r = lambda lo, hi: int(torch.randint(lo, hi + 1, (1,), generator=g))  # noqa: E731
+    sizes = [(1 if r(0, 2) else r(2, 63), 0) for _ in range(9)] + [(63, 0)]
+    sizes = [(n, n + r(200, 3000)) for n, _ in sizes]
+    c = Cache(fmt, rows, 8, hd, n_seqs=10, max_len=3100, page=64, seed=hd + 5)
+    for s in range(10):
+        c.scale["v"][c.table_cpu[s].long().cuda()] *= 2.0 ** (3 if s % 2 else -3)
+    masks = [1 << j | (1 << max(0, j - 3)) | 1 for n, _ in sizes for j in range(n)]
+    _both(backend, c, sizes, 64, seed=seed, masks=masks)
