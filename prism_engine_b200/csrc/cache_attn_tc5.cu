@@ -684,18 +684,20 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         }
         float m = -INFINITY, l = 0.0f;
         int32_t ref = 0;                                           // exponent that O is over
+        // A warp that had no rows in the parts before may be phases ahead of the slots of scales, and parity would let it read an older tile's
+        // exponent.  So it waits for the first scores, which follow their scales, and from then on is in step.  (Scores before scales in every
+        // tile: 588 instead of 567 us for 28 heads of 128 over 4, 2 x 2048 tokens over 6001 positions, int4.)
+        if (CODES && mine) t5::mbar_wait_warp(b_sfull + 8 * q, Tq & 1, err_flag);
         for (uint32_t j = 0; j < mine; j++) {
             int32_t ex = 0;
             const float *ksc = nullptr;
-            t5::mbar_wait_warp(b_sfull + 8 * q, (Tq + j) & 1, err_flag);
             if constexpr (CODES) {
-                // After the scores, which follow these scales: before them a warp that had no rows in the parts before could be phases ahead of
-                // the slot, and parity would let it read an older tile's.  The wait passes at once, and makes the scales visible.
                 t5::mbar_wait_warp(b_sc + 8 * ((T + j) % CT_SC), ((T + j) / CT_SC) & 1, err_flag);
                 ksc = reinterpret_cast<const float *>(sm + C::SC_OFF + ((T + j) % CT_SC) * C::SLOT);
                 ex = ct_exponent(ksc + 2 * CT_POS * NSC);
                 ksc += half * 64;                                  // scales of all positions, then zeros
             }
+            t5::mbar_wait_warp(b_sfull + 8 * q, (Tq + j) & 1, err_flag);
             t5::fence_after();
             uint32_t s[2][32];
 #pragma unroll
@@ -945,10 +947,10 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         }
         uint4 reg[MINE];
         float2 scr[2][2];                                          // keys', values' scales of positions ct and ct + 96
-        // lanes 0..7: the pool row of the tile's 16-position unit; NO_PAGE where there is none: the scales of its keys are NaN, so that the rows
-        // that look at them are taken again, which skips them
-        uint32_t at_k = 0, at_v = 0;
-        constexpr uint32_t NO_PAGE = 0x80000000u;
+        uint32_t at_k = 0, at_v = 0;                               // lanes 0..7: the pool row of the tile's 16-position unit (0 where there is none)
+        // a bit for each unit of at_k: somebody looks at it, and it has a page or not (none: the scales of its keys are NaN, so that the rows that
+        // look at it are taken again, which skips it)
+        uint32_t some = 0, none = 0;
         // Pages are asked for two tiles ahead, so that nothing waits for the table.
         auto look = [&](const CtSegment &g, uint32_t j) {
             const int32_t p = j < g.n ? pos_of(g, j) + (int32_t)(lane & 7) * 16 : 0;
@@ -956,8 +958,10 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         };
         auto units = [&](const CtSegment &g, uint32_t j, uint32_t page) {
             const int32_t p = j < g.n ? pos_of(g, j) + (int32_t)(lane & 7) * 16 : 0;
-            if (j >= g.n || !wanted(g, p, 16)) return 0u;
-            return kv_page_ok(a.c, page) ? (uint32_t)kv_row(a.c, page, g.kh, (uint32_t)p) : NO_PAGE;
+            const bool want = j < g.n && wanted(g, p, 16), ok = want && kv_page_ok(a.c, page);
+            some = __ballot_sync(0xFFFFFFFFu, ok);
+            none = __ballot_sync(0xFFFFFFFFu, want && !ok);
+            return ok ? (uint32_t)kv_row(a.c, page, g.kh, (uint32_t)p) : 0u;
         };
         uint32_t page;
         // Four pieces at a time, so that what they wait for overlaps.
@@ -965,7 +969,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
         auto load = [&](const uint8_t *pool, int first, uint32_t of) {
             uint32_t at[G];
 #pragma unroll
-            for (int i = 0; i < G; i++) at[i] = __shfl_sync(0xFFFFFFFFu, of, ((row0 + (first + i) * STEP) >> 4) & 7) & ~NO_PAGE;
+            for (int i = 0; i < G; i++) at[i] = __shfl_sync(0xFFFFFFFFu, of, ((row0 + (first + i) * STEP) >> 4) & 7);
 #pragma unroll
             for (int i = 0; i < G; i++)
                 if (first + i < MINE) reg[first + i] = t5::ldg128_nc(pool + (size_t)(at[i] + ((row0 + (first + i) * STEP) & 15)) * C::ROWB + piece * 16);
@@ -981,14 +985,13 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             }
         };
         constexpr int FULL = CT_POS / STEP;                        // pieces that every thread has
-        auto load_scales = [&](const CtSegment &g, int32_t p0, uint32_t of) {
+        auto load_scales = [&](int32_t p0, int32_t len, uint32_t of) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const uint32_t row = ct + h * 96, at = __shfl_sync(0xFFFFFFFFu, of, (row >> 4) & 7);
-                scr[0][h] = scr[1][h] = make_float2(0.0f, 0.0f);
-                if (at & NO_PAGE) {
-                    scr[0][h].x = __uint_as_float(0x7FC00000u);
-                } else if (row < CT_POS && p0 + (int32_t)row < g.x.len && wanted(g, p0 + (int32_t)(row & ~15u), 16)) {
+                scr[0][h] = make_float2(none >> (row >> 4) & 1 ? __uint_as_float(0x7FC00000u) : 0.0f, 0.0f);
+                scr[1][h] = make_float2(0.0f, 0.0f);
+                if ((some >> (row >> 4) & 1) && row < CT_POS && p0 + (int32_t)row < len) {
                     const size_t from = ((size_t)at + (row & 15)) * NSC;
                     if constexpr (NSC == 2) {
                         scr[0][h] = __ldg(reinterpret_cast<const float2 *>(a.c.ks + from));
@@ -1010,7 +1013,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             page = look(g, 1);
 #pragma unroll
             for (int i = 0; i < MINE; i += G) load(a.c.k, i, at_k);
-            load_scales(g, pos_of(g, 0), at_k);
+            load_scales(pos_of(g, 0), g.x.len, at_k);
         }
         for (uint32_t j = 0; j < n; j++) {
             const uint32_t st = (T + j) % ST, ph = ((T + j) / ST) & 1;
@@ -1060,7 +1063,7 @@ __global__ void __launch_bounds__(CtCfg<KIND, HD>::THREADS, 1) cache_tiles_kerne
             }
             at_k = units(g, j + 1, page);
             page = look(g, j + 2);
-            load_scales(g, next, at_k);
+            load_scales(next, g.x.len, at_k);
             const uint32_t kt = base + C::K_OFF + st * C::TILE, vt = base + C::V_OFF + st * C::TILE;
             clear(g, now);
 #pragma unroll
