@@ -297,11 +297,11 @@ int prism_cuda_attention_step_kv(prism_cuda_ctx *ctx, uint32_t layer, const uint
  *   PRISM_CACHE_INT4    value = (code - 8) * scale + zero, scale = (hi - lo) / 15,   code = rint((x - lo) * (15 / (hi - lo))),
  *                       zero = lo + 8 * scale; element 2i in the low half of byte i
  * amax, lo, hi: over one head of one position; every step one rounded 32-bit operation.  A span below 2^-100 gives scale 0; a
- * head with a value that is not finite reads back as NaN throughout.
- * Pages, scales and rows are 16-byte aligned device memory, arrays of 32-bit numbers 4-byte aligned.  The calls run on the context's stream and return; places are in
- * device arrays, so a captured call can be replayed with others.  A place outside the cache, or whose page is not one of the
- * pool's, is skipped, and the next synchronising call returns PRISM_E_ARG; a negative sequence or position is padding and
- * skipped without that. */
+ * head of codes with a value, or at 4 bits a span, that is not finite reads back as NaN throughout.
+ * Pages, scales and rows are 16-byte aligned device memory, arrays of 32-bit numbers 4-byte aligned.  The calls run on the
+ * context's stream and return; places are in device arrays, so a captured call can be replayed with others.  A place outside the
+ * cache, or whose page is not one of the pool's, is skipped, and the next synchronising call returns PRISM_E_ARG; a negative
+ * sequence or position is padding and skipped without that. */
 enum { PRISM_CACHE_16BIT = 0, PRISM_CACHE_INT8 = 1, PRISM_CACHE_E4M3 = 2, PRISM_CACHE_INT4 = 3 };
 enum { PRISM_CACHE_ROWS_F16 = 0, PRISM_CACHE_ROWS_BF16 = 1 };
 typedef struct prism_cache {
@@ -337,8 +337,11 @@ int prism_cuda_cache_keep_dev(prism_cuda_ctx *ctx, const prism_cache *cache, uin
  * With a tree the rows are drafted tokens of equal standing: row i of the entry lies at position length[e] - n + i of the cache and sees
  * the drafted position j of its own entry if bit j of its mask (tree[row * tree_words], 64 bits a word) is set; of the committed
  * positions c < length[e] - n it sees those that window and sinks leave to a token at q_pos[row].
- * Query heads are shared evenly by the cached ones.  out = sum of softmax(scale * q k) v, scores, weights' sums and result in 32
- * bits; a row that sees nothing is 0, rows of no entry (and of an entry with a negative sequence) are left as they were. */
+ * Query heads are shared evenly by the cached ones.  out = sum of softmax(scale * q k) v, scores and all sums in 32 bits, products
+ * of 16-bit operands (weights, and coded values and queries over powers of two, are rounded to 16 bits once), one rounding at the
+ * end; a row that sees nothing is 0, rows of no entry (and of an entry with a negative sequence) are left as they were.  Pages of which no
+ * row sees a position are not looked at: their numbers may be anything.  Rows that meet values that are not finite, bad pages, or
+ * many together over codes whose values lie more than 2^16 apart, are taken one by one in 32 bits, which is slower by far. */
 typedef struct prism_cache_attention {
     const void *q;           /* rows of num_heads * head_dim values */
     void *out;               /* overlaps neither q nor the cache */

@@ -328,7 +328,8 @@ class CudaBackend:
         ``q_start[e] .. q_start[e + 1]`` of ``q`` and ``out`` over the first ``length[e]`` positions of sequence ``seq[e]``; under a
         ``window`` a row sees that many positions up to its own and the first ``sinks``.  ``tree``: 64-bit masks (``tree_words`` a
         row) of the drafted tokens of its entry that each row sees, itself included; ``q_pos``: the rows' positions, which a window
-        over the committed ones goes by.  ``scale`` 0: 1 / sqrt(head_dim).  ``out`` overlaps neither ``q`` nor the cache."""
+        over the committed ones goes by.  ``scale`` 0: 1 / sqrt(head_dim).  ``out`` overlaps neither ``q`` nor the cache.  Pages of
+        which no row sees a position are not looked at, their numbers may be anything."""
         w = num_heads * cache.head_dim
         a = CacheAttention(q, out, q_stride or w, out_stride or w, n_rows, n_entries, seq, q_start, length, max_tokens, max_length, num_heads,
                            window, sinks, scale, tree or None, tree_words, q_pos or None)

@@ -11,7 +11,9 @@
 //   score = (q c) ks + (sum of q) kz,     o = sum of (w vs) c + sum of w vz.
 // w vs enters the product as fp16 over the power of two below the row's largest so far, 2^14-fold, so no scale over- or underflows;
 // with 16-bit rows w itself does (fp16: 2^13-fold, bf16: as it is), and the sum that divides is that of the rounded weights.  q of 8- and 4-bit caches enters
-// as fp16 over a power of two.  Maxima, sums, O and everything that multiplies them are 32 bits.
+// as fp16 over a power of two.  Maxima, sums, O and everything that multiplies them are 32 bits.  The 16 bits are what the products
+// take: a weight is rounded once (2^-8 of itself in bf16, 2^-11 in fp16), as the result is, and q over a power of two keeps its bits but for elements
+// 2^-14 of its largest.
 //
 // Positions past the end are zero.  A position that some row of the block does not see meets weight 0, which an infinity there turns into
 // NaN: a row whose result is not finite is taken again by itself (cache_plain_row).
@@ -20,8 +22,8 @@
 // the shared memory of all (through scratch and a counter: 14 heads of 64 over 711 positions 9.0 us, by clusters 5.5); more go through scratch to cache_join_kernel.
 // Bound: HBM for long caches of 16-bit rows; the instructions about codes (some 850 a warp for 32 positions of a 128-wide head: places, copies, bytes to
 // fragments, scales, softmax) at 8 and 4 bits; the latency of the chain (places, tiles, joining) for short ones.
-// 64 heads of 128 over 8, a token of 32 sequences under a window of 4096: 16 bits 85 us (6.3 TB/s), int8 63 us (4.4 TB/s), int4 64 us; one sequence of 131071
-// positions: 16 bits 93 us (5.8 TB/s), int4 56 us (2.7 TB/s); 14 heads of 64 over 2, 516 visible positions: 5.5 us.
+// 64 heads of 128 over 8, a token of 32 sequences under a window of 4096: 16 bits 85 us (6.3 TB/s), int8 63 us (4.4 TB/s), int4 65 us; one sequence of 131071
+// positions: 16 bits 91 us (5.9 TB/s), int4 56 us (2.7 TB/s); 14 heads of 64 over 2, 516 visible positions: 5.5 us.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -38,7 +40,7 @@ constexpr uint32_t CR_CLUSTER = 8;               // parts whose blocks are a clu
 constexpr uint32_t CR_NEAR = 512;                // positions of a part
 // More than 32 rows of a cached head are for the tcgen05 kernel, whose blocks cost 6 us more to begin and to end, where 16-row tiles are more than
 // two an SM or tiles times positions more than this.  8 cached heads of 128, 64 to 256 rows (int8): one sequence of 2000 positions 12 to 25 us here,
-// 20 to 24 there; eight of 711 20 to 75 here, 25 to 34 there; eight of 8000 149 to 559 here, 130 to 146 there.  To 32 rows this one always:
+// 20 to 26 there; eight of 711 20 to 76 here, 27 to 35 there; eight of 8000 127 to 479 here, 134 to 151 there.  To 32 rows this one always:
 // eight of 8000 positions, 32 rows: int8 71 us here, 128 there, 16 bits 68 and 75.
 constexpr uint64_t CR_WORK = 200000;
 constexpr float CR_UP = 16384.0f;                // weights of fp16 products of codes are 2^14-fold, and below 2; of fp16 rows 2^13-fold, and below 2^CR_GROW

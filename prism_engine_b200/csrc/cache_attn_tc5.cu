@@ -13,6 +13,11 @@
 //                 by the exponent in which its tile lies below the largest so far.  Where positions' values lie more than 2^16 apart, seen or
 //                 not, the rows are taken by themselves.
 //
+// Why 16 bits where they are: the products take 16-bit operands at twice the rate of 32-bit ones, from tiles of half the size.  A weight is
+// rounded once, to the rows' type or fp16 (2^-8 or 2^-11 of itself), as the result is; q over a power of two keeps its bits but for elements 2^-14 of
+// its largest; a coded value is rounded once to fp16 (2^-11), where its scale kept apart would have to go into each row's weight.  The polynomial of a
+// quarter of the 16-bit exponentials is off by 2.6e-6, far below the rounding of the weight that follows.  Scores, maxima, sums and O are 32 bits.
+//
 // Positions past the end are zero.  A position that a row does not see meets weight 0, which an infinity there turns into NaN: a row whose
 // result is not finite is taken again by itself (cache_plain_row), after all parts of its block.
 // Few row tiles: the positions are cut into parts whose fp32 sums cache_join_kernel joins in order.  More of them: the blocks, one an SM, share
@@ -20,8 +25,8 @@
 // Bound: the tensor core and the instructions about the scores together: 2 048 cycles of products for 256 rows and 128 positions of a 128-wide head,
 // as many for their exponentials, and some 5 instructions a score (codes: 6 to 7) on four schedulers; a tile takes 4 300 cycles of 16-bit rows.
 // Besides, 15 000 cycles a row tile: q, the first products, results.
-// 28 heads of 128 over 4, 2 x 2048 tokens over 6001 positions, bf16: 306 us (0.96 PFLOP/s), under a window of 1024 123 us; int8 508 us.  8 x 63 drafted
-// tokens of 64 heads over 4100 positions: int8 94 us, 16 bits 74 us.
+// 28 heads of 128 over 4, 2 x 2048 tokens over 6001 positions, bf16: 316 us (0.92 PFLOP/s), under a window of 1024 129 us; int8 535 us, int4
+// 570 us.  8 x 63 drafted tokens of 64 heads over 4100 positions: int8 99 us, 16 bits 76 us.
 #include <algorithm>
 
 #include "cache_join.cuh"
@@ -289,14 +294,14 @@ __device__ __forceinline__ void ct_convert(uint32_t tile, uint32_t flip, const u
     }
 }
 
-// The results of a row tile's part that this thread's row has, half of the columns: stored, or left as a part, which the last block to arrive joins.
-// A function of its own: inlined into the loop over parts it took some 350 registers more than there are.
 // Where 16-byte piece c of a row of q lies.
 template <int HD>
 __device__ __forceinline__ uint8_t *ct_q_piece(uint8_t *sm, uint32_t q, uint32_t row, uint32_t c) {
     return sm + q * CtCfg<KV_F16, HD>::TILE + (c >> 3) * CtCfg<KV_F16, HD>::PANEL + row * 128 + (((c & 7) ^ (row & 7)) << 4);
 }
 
+// The results of a row tile's part that this thread's row has, half of the columns: stored, or left as a part, which the last block to arrive joins.
+// A function of its own: inlined into the loop over parts it took some 350 registers more than there are.
 template <int KIND, int HD>
 __device__ __noinline__ void ct_results(const CtDev &d, CtSegment &g, uint8_t *sm, uint32_t o_col, uint32_t warp, uint32_t lane, uint32_t mine, float m,
                                         float l, int32_t ref) {

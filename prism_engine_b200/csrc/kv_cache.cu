@@ -10,10 +10,11 @@
 //
 // hd / 16 lanes share a head of a position (a unit), 8 values from each half of it a lane, so loads and stores are whole lines and the extremes take
 // log2(hd / 16) shuffles; a task is two units of one row.  Codes are rounded by adding 1.5 * 2^23, whose last bits they then are, and gathered by
-// byte permutes.  Bound: HBM for long lists (the dependent look-ups of place and page in front of a task's data, and the instructions of the
-// divisions, are what is left of it), launch latency for a decode step's rows.
-// Reading up to 6 x 8000 rows of 8 heads of 128: from e4m3 37.5 us (4.8 TB/s), from 16 bits 38.9 (6.1 TB/s); four units a task 43.5 and 41.3, one
-// 38.1 and 42.0.  Writing up to 4 x 2048 rows of them in int4 15.8 us (3.8 TB/s); four units 16.8, one 16.5.
+// byte permutes.  Bound: HBM for long lists of 16-bit rows; for codes the time goes by tasks, not by bytes (a thread group does one, with its place,
+// page and data in turn, and ends); launch latency for a decode step's rows.
+// Reading up to 6 x 8000 rows of 8 heads of 128: from 16 bits 38.7 us (6.3 TB/s), e4m3 37.5 (4.9 TB/s), int4 36.6; four units a task 43.5 from e4m3
+// and 41.3 from 16 bits, one 38.1 and 42.0.  Up to 4 x 2048 such rows, which L2 holds: written in 16 bits 5.4 us, int8 7.4, e4m3 7.1, int4 9.0 (3.4 TB/s),
+// written in int4 and read back 15.7; four units 16.8, one 16.5.
 #include <stdexcept>
 
 #include "kv_cache.cuh"
