@@ -339,9 +339,10 @@ int prism_cuda_cache_keep_dev(prism_cuda_ctx *ctx, const prism_cache *cache, uin
  * positions c < length[e] - n it sees those that window and sinks leave to a token at q_pos[row].
  * Query heads are shared evenly by the cached ones.  out = sum of softmax(scale * q k) v, scores and all sums in 32 bits, products
  * of 16-bit operands (weights, and coded values and queries over powers of two, are rounded to 16 bits once), one rounding at the
- * end; a row that sees nothing is 0, rows of no entry (and of an entry with a negative sequence) are left as they were.  Pages of which no
- * row sees a position are not looked at: their numbers may be anything.  Rows that meet values that are not finite, bad pages, or
- * many together over codes whose values lie more than 2^16 apart, are taken one by one in 32 bits, which is slower by far. */
+ * end; a row that sees nothing is 0, rows of no entry (and of an entry with a negative sequence) are left as they were.
+ * Pages of which no row sees a position are not looked at: their numbers may be anything.  Rows that meet values that are not
+ * finite, bad pages, or many together over codes whose values lie more than 2^16 apart, are taken one by one in 32 bits, which is
+ * slower by far. */
 typedef struct prism_cache_attention {
     const void *q;           /* rows of num_heads * head_dim values */
     void *out;               /* overlaps neither q nor the cache */

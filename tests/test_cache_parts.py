@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from cache_parts import parts
-from cache_util import Cache, check, queries, run_attention
+from cache_util import Cache, check, i32, queries, run_attention
 from test_gpu_cache_many_rows import _both, _entries, oracle
 
 SMS = 148  # blocks that share the work
@@ -172,3 +172,31 @@ def test_ragged_drafts_over_codes(backend, fmt, rows, hd, seed):
         c.scale["v"][c.table_cpu[s].long().cuda()] *= 2.0 ** (3 if s % 2 else -3)
     masks = [1 << j | (1 << max(0, j - 3)) | 1 for n, _ in sizes for j in range(n)]
     _both(backend, c, sizes, 64, seed=seed, masks=masks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,rows,hd", KINDS16 + CODED[:3])
+def test_rows_apart_and_padding_between_entries(backend, fmt, rows, hd):
+    """Queries and results with gaps between rows, entries of a negative sequence and without rows among the others: what belongs to no
+    entry stays as it was."""
+    sizes = [(40 - i, 400 + 9 * i) if i % 7 else (0, 50) for i in range(30)]
+    c = Cache(fmt, rows, 2, hd, n_seqs=6, max_len=700, page=64, seed=hd + 6)
+    entries, n = _entries(sizes, [i % 6 for i in range(30)])
+    q = queries(n + 5, 16, hd, rows, 7)
+    padding = [i % 5 == 3 for i in range(30)]
+    want, tol = oracle(c, q, [e for e, p in zip(entries, padding) if not p], 16, window=200, sinks=7)
+    wide = torch.full((n + 5, 3, 16, hd), 7.0, dtype=q.dtype, device="cuda")
+    wide[:, 1] = q.cuda()
+    a = [i32([-1 if p else e[0] for e, p in zip(entries, padding)]), i32([e[1] for e in entries] + [n]), i32([e[3] for e in entries])]
+    torch.cuda.synchronize()
+    step, row = 3 * 16 * hd, 16 * hd * 2
+    backend.cache_attention_dev(c.view(), wide.data_ptr() + row, wide.data_ptr() + 2 * row, n_rows=n + 5, n_entries=30, seq=a[0].data_ptr(),
+                                q_start=a[1].data_ptr(), length=a[2].data_ptr(), max_tokens=40, max_length=700, num_heads=16, window=200, sinks=7,
+                                q_stride=step, out_stride=step)
+    backend.synchronize()
+    theirs = torch.zeros(n + 5, dtype=torch.bool)
+    for (_, r0, t, _), p in zip(entries, padding):
+        theirs[r0:r0 + t] = not p
+    got = wide.cpu()
+    check(got[:, 2], want, tol, theirs)
+    assert (got[~theirs][:, 2] == 7).all() and (got[:, 0] == 7).all() and torch.equal(got[:, 1], q)
